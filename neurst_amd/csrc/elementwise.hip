@@ -332,7 +332,11 @@ __global__ void adam_kernel(float* __restrict__ p, const float* __restrict__ g, 
     for (int j = 0; j < 4; ++j) {
       float gj = gg[e][j] * gs;
       mm[e][j] = b1 * mm[e][j] + (1.f - b1) * gj;
-      vv[e][j] = b2 * vv[e][j] + (1.f - b2) * gj * gj;
+      {
+        // products and sum rounded one by one: a fused form moves v by a last bit from what it always was here
+#pragma clang fp contract(off)
+        vv[e][j] = b2 * vv[e][j] + (1.f - b2) * gj * gj;
+      }
       pp[e][j] = pp[e][j] - lr_t * mm[e][j] / (sqrtf(vv[e][j]) + eps);
       sh[j] = (bf16_t)pp[e][j];
     }
