@@ -404,6 +404,70 @@ int neurst_beam_prune(const float* next_scores, const int32_t* next_ids, const f
 int neurst_gather_rows(const void* src, void* dst, const int32_t* idx, int64_t rows, int64_t row_bytes, int64_t src_stride,
                        int64_t dst_stride, void* stream);
 
+/* ---- paged decoding: operators next to the cached decoder (st/models/decoders/transformer_decoder.py:52-182) that the
+ * reference has no counterpart of: positions by rotation, a key/value cache of pages, attention of a chunk of new tokens
+ * over it, drawing the next token. ----
+ *
+ * Rotary positions: y = x with the first 2 * pairs columns of each head turned by the row's position.  Pair i at position p:
+ *   u' = mscale (u cos a - v sin a), v' = mscale (v cos a + u sin a), a = p * freq[i] (fp64 inside: exact to 2^-33 turns),
+ * the pair being columns (i, pairs + i) (layout 0, "half") or (2 i, 2 i + 1) (layout 1, "interleaved"); further columns
+ * pass through.  x, y: rows of `heads` heads of dh columns at row strides ldx / ldy (elements); y may be x.  positions
+ * int32 [rows], or NULL: row r stands at pos0 + (period ? r % period : r).  inverse != 0 turns back: the gradient. */
+int neurst_rotary(const void* x, void* y, const double* freq, const int32_t* positions, int64_t rows, int64_t heads,
+                  int64_t dh, int64_t pairs, int64_t ldx, int64_t ldy, int64_t pos0, int64_t period, int layout, int inverse,
+                  float mscale, int dtype, void* stream);
+
+/* The paged cache.  k_pages [n_pages][kv_heads][page_size][dh], v_pages TRANSPOSED [n_pages][kv_heads][dh][page_size]
+ * (page_size a power of two in 16..4096, dh a multiple of 8 up to 256; both 16-byte aligned).  page_table int32 [batch][wide]
+ * (row stride ld_table, 0: one row for all): position p of sequence b lives in page page_table[b][p / page_size], slot p % page_size; sequences
+ * may share pages that none of them writes.  A call's `tokens` new rows are packed by sequence: cu_new int32 [batch + 1],
+ * sequence b owns rows cu_new[b] .. cu_new[b + 1] - 1 (none is fine); ctx_len int32 [batch] = tokens in its cache WITH them, so
+ * its row j stands at position ctx_len[b] - n_b + j.  Rows of no sequence are left as they are.
+ *
+ * These arrays live on the device.  A kernel that finds lengths that do not fit (rows out of range, ctx_len < n_b or
+ * beyond the table) or a page id outside the pool leaves that sequence or those keys out, and ors 2 or 1 into *status (may
+ * be NULL); it reads and writes nothing out of range.
+ *
+ * neurst_paged_append writes the new keys k (rotated by position when freq is not NULL: pairs, layout, mscale as above) and
+ *   values v into their pages and, when q is not NULL, the rotated queries to q_out (may be q).
+ * neurst_paged_attention: o = softmax(scale q . k^T) v per query head over the keys 0 .. position (causal != 0) or all
+ *   ctx_len[b]; query head h reads key/value head h / (q_heads / kv_heads).  A row that sees nothing gets zeros.  Masked keys
+ *   never reach a result, whatever they hold.  workspace: neurst_paged_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ *   of this call alone until it has run. */
+int neurst_paged_append(const void* k, const void* v, const void* q, void* k_pages, void* v_pages, void* q_out,
+                        const int32_t* page_table, const int32_t* cu_new, const int32_t* ctx_len, const double* freq,
+                        int32_t* status, int64_t tokens, int64_t batch, int64_t wide, int64_t ld_table, int64_t n_pages,
+                        int64_t page_size, int64_t kv_heads, int64_t q_heads, int64_t dh, int64_t ldk, int64_t ldv,
+                        int64_t ldq, int64_t ldqo, int64_t pairs, int layout, float mscale, int dtype, void* stream);
+int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size,
+                                               int64_t q_heads, int64_t kv_heads, int64_t dh, int dtype);
+int neurst_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                           const int32_t* cu_new, const int32_t* ctx_len, int32_t* status, int64_t tokens, int64_t batch,
+                           int64_t wide, int64_t ld_table, int64_t n_pages, int64_t page_size, int64_t q_heads,
+                           int64_t kv_heads, int64_t dh, int64_t ldq, int64_t ldo, float scale, int causal, int dtype,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Draws one token per row of logits [rows][V] (row stride ld; fp32 or bf16; V <= 524288) from a given u in [0, 1) per row:
+ *   w_i = exp((l_i - max l) / temperature), rounded to whole multiples of 2^-44; keep the top_k largest (0: all; equal ones: lower index first), of these the
+ *   shortest leading run in descending order whose sum reaches top_p of theirs, of these the ones with w_i >= min_p;
+ *   ids = the first kept index, in index order, whose running sum exceeds u times the kept sum; logp = log(w_id / kept sum).
+ * temperature 0 (or a top_k of 1): the first maximum.  NaN and -inf logits are never drawn; a row of nothing else gives id
+ * -1, logp -inf.  The weights being integers, sums are exact and a draw is the same whatever the launch; a word below 2^-45
+ * of the best is never drawn.  *_rows (may
+ * be NULL): one parameter per row, device arrays; out-of-range values there mean "off" (top_k <= 0, NaN min_p), the arg-max
+ * (temperature not above 0) or the nearest allowed value.
+ * neurst_sample_step draws and keeps a decoding step's books the way neurst_greedy_step does: tokens [rows] = preds[r, step] =
+ *   the draw (eos for a finished row or one with nothing to draw), finished |= token == eos, len_decoded += 1 - finished,
+ *   n_unfinished += !finished, scores += logp while unfinished. */
+int neurst_sample(const void* logits, const float* u, int32_t* ids, float* logp, const float* temperature_rows,
+                  const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, float temperature, int top_k,
+                  float top_p, float min_p, int64_t rows, int64_t V, int64_t ld, int dtype, void* stream);
+int neurst_sample_step(const void* logits, const float* u, int32_t* tokens, int32_t* preds, int32_t* finished,
+                       int32_t* len_decoded, int32_t* n_unfinished, float* scores, const float* temperature_rows,
+                       const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, float temperature,
+                       int top_k, float top_p, float min_p, int64_t rows, int64_t V, int64_t ld, int64_t step,
+                       int64_t max_steps, int eos, int dtype, void* stream);
+
 /* Input pipeline, host side (pure host code, callable without a GPU).  Replaces what the reference
  * gets from TensorFlow's tf.TFRecordReader / tf.parse_single_example / tf.python_io.TFRecordWriter
  * (st/tools/tftools/tfRecord.py:107-150 writer, :460-824 readers; `*.recode` files, :848-855).

@@ -1,0 +1,375 @@
+// Attention of a chunk of new tokens over the paged key/value cache (paged.hip has the layout):
+//
+//   o[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / group]) v[j, h / group],   j = 0 .. p_i (causal) or 0 .. ctx - 1
+//
+// over all new tokens i of all sequences, p_i the token's position.  One pass with the running maximum and sum; the table of
+// weights never exists.  A token that sees nothing gets zeros.  No reference counterpart in this form: decoding there re-runs
+// st/layers/common_attention_v1.py:325-365 on dense caches of equal length.
+//
+// paged_attn_rows: few rows (single tokens, short chunks).  A workgroup owns 16 rows - tokens x the query heads that share a
+// key/value head - and its waves take tiles of 32 keys (fp32: 16) in turn, straight from the pages to the matrix
+// instructions.  The first product is taken transposed, S^T = K Q^T, with the keys of a tile dealt to the rows of the
+// instruction such that a lane's results are eight CONSECUTIVE keys of one query: after exp2 and the rounding to bf16 they
+// are, in place, the operand of O^T = V^T P^T, whose other operand is one 16-byte load from the transposed value pages.  No
+// shared memory and no barrier until the waves join their partial results.
+#include "paged.h"
+
+struct PagedAttnArgs {
+  PagedIndex ix;
+  const void *q, *k_pages, *v_pages;
+  void* o;
+  float *ws_o, *ws_ml;      // splits > 1: partial results [split][row][dh padded], [split][row][2]
+  int32_t* status;
+  int64_t ldq, ldo;
+  int hkv, group, dh, causal, splits;
+  float scale_log2;         // scale * log2(e): exp(x) = exp2(x log2(e))
+};
+
+template <typename T> struct PagedMma;
+template <> struct PagedMma<bf16_t> {
+  static constexpr int E = 8, KT = 32, NSUB = 2;      // elements of a 16-byte load, keys of a tile, 16-key halves
+  typedef bf16x8 V;
+  static __device__ __forceinline__ f32x4 mma(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct PagedMma<float> {
+  static constexpr int E = 4, KT = 16, NSUB = 1;
+  typedef f32x4 V;
+  static __device__ __forceinline__ f32x4 mma(V a, V b, f32x4 c) {      // four steps of the 4-deep instruction
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// exp2(m_old - m_new) where -inf stands for "nothing yet"
+__device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// what a workgroup of `tile` works on; false: nothing
+struct RowTile {
+  int b, first_token, last_token, n_rows, kv_end, min_vis;   // keys 0 .. kv_end - 1 are visible to some row, 0 .. min_vis - 1 to every row
+  int64_t row0;
+  int shift;                                                  // position of token 0
+  int row_begin;                                              // first of the tile's rows within the sequence
+};
+template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs& a, int64_t tile, int lane, RowTile& t, bool report) {
+  t.b = paged_find(a.ix, tile, a.group, ROWS, 1, lane);
+  if (t.b < 0) return false;
+  const PagedSeq s = paged_seq(a.ix, t.b);
+  if (report && s.bad) paged_report(a.status, s.bad);
+  const int64_t own = tile - paged_tile_start(a.ix.cu[t.b], a.group, ROWS, 1, t.b);
+  const int64_t rows = (int64_t)s.new_tokens * a.group;
+  if (own * ROWS >= rows) return false;
+  t.row_begin = (int)(own * ROWS);
+  t.n_rows = (int)(rows - own * ROWS < ROWS ? rows - own * ROWS : ROWS);
+  t.row0 = s.row0;
+  t.first_token = t.row_begin / a.group;
+  t.last_token = (t.row_begin + t.n_rows - 1) / a.group;
+  t.shift = s.ctx - s.new_tokens;
+  if (s.ctx == 0) { t.kv_end = t.min_vis = 0; t.shift = -1; }
+  else if (a.causal) { t.kv_end = t.shift + t.last_token + 1; t.min_vis = t.shift + t.first_token + 1; }
+  else t.kv_end = t.min_vis = s.ctx;
+  return true;
+}
+
+template <typename T, int DH, bool EXACT, int NW>
+__global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
+  typedef PagedMma<T> A;
+  typedef typename A::V V;
+  constexpr int E = A::E, KT = A::KT, NSUB = A::NSUB, KC = DH / (4 * E), ND = DH / 16;
+  constexpr int NDP = ND < 8 ? ND : 8, LD = NDP * 16 + 4;      // dims joined at a time through LDS
+  __shared__ float red[NW][16][LD];
+  __shared__ float ml[NW][16][2];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, z = blockIdx.z;
+  RowTile t;
+  if (!row_tile<16>(a, blockIdx.x, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  const int dh = EXACT ? DH : a.dh;
+  const int page = 1 << a.ix.page_log2, pmask = page - 1;
+  // this lane's query: row m of the tile
+  const bool valid = m < t.n_rows;
+  const int r = t.row_begin + (valid ? m : 0), token = r / a.group, head = kvh * a.group + r % a.group;
+  const T* qp = static_cast<const T*>(a.q) + (t.row0 + token) * a.ldq + (int64_t)head * dh;
+  V qf[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) {
+    const int d = c * 4 * E + E * g;
+    if (EXACT || d < dh) qf[c] = *reinterpret_cast<const V*>(qp + d);
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) qf[c][e] = (T)0.f;
+  }
+  const int vis = a.causal ? (t.kv_end ? t.shift + token + 1 : 0) : t.kv_end;
+  // this split's tiles
+  const int nt = (t.kv_end + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits;
+  const int t0 = z * per, t1 = t0 + per < nt ? t0 + per : nt;
+
+  f32x4 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float mx = -INFINITY, l = 0.f;
+  for (int ti = t0 + w; ti < t1; ti += NW) {
+    const int base = ti * KT;
+    // pages of the E-key groups this lane reads: keys of group m >> 2 for the first product, of group g for the second
+    const int kg = base + E * (m >> 2), vg = base + E * g;
+    const int kp = kg < t.kv_end ? paged_page(a.ix, t.b, kg) : -1;
+    const int vp = vg < t.kv_end ? paged_page(a.ix, t.b, vg) : -1;
+    if (vp < 0 && vg < t.kv_end) paged_report(a.status, PAGED_BAD_PAGE);
+    const bool full = base + KT <= t.min_vis && __all(vp >= 0);
+    const T* kb = static_cast<const T*>(a.k_pages) +
+                  (((((int64_t)(kp < 0 ? 0 : kp) * a.hkv + kvh) << a.ix.page_log2) + (kg & pmask) + (m & 3)) * dh);
+    const T* vb = static_cast<const T*>(a.v_pages) + ((((int64_t)(vp < 0 ? 0 : vp) * a.hkv + kvh) * dh << a.ix.page_log2) + (vg & pmask));
+    V kf[NSUB][KC], vf[ND];
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int d = c * 4 * E + E * g;
+        kf[s][c] = *reinterpret_cast<const V*>(kb + (int64_t)4 * s * dh + (EXACT || d < dh ? d : 0));
+      }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int dim = 16 * d + m;
+      vf[d] = *reinterpret_cast<const V*>(vb + ((int64_t)(EXACT || dim < dh ? dim : 0) << a.ix.page_log2));
+    }
+    f32x4 sc[NSUB];
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) {
+      sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        V k = kf[s][c];
+        if (!EXACT && c * 4 * E + E * g >= dh)
+#pragma unroll
+          for (int e = 0; e < E; ++e) k[e] = (T)0.f;
+        sc[s] = A::mma(k, qf[c], sc[s]);
+      }
+    }
+    float x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = sc[e >> 2][e & 3] * a.scale_log2;     // keys vg + e of query m
+    if (!full) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (vp < 0 || vg + e >= vis) x[e] = -INFINITY;
+    }
+    float tm = x[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) tm = fmaxf(tm, x[e]);
+    tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+    const float mn = fmaxf(mx, tm), mu = safe_max(mn);
+    if (__any(mn > mx)) {
+      const float al = fast_exp2(mx - mu);       // 0 while mx is -inf
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= al;
+      mx = mn;
+    }
+    // the weights are rounded to the values' type for the second product (bf16: a relative 2^-9 of each, the plain form's
+    // own rounding of the output is as large); their sum is taken before that, in fp32
+    V p;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float pe = fast_exp2(x[e] - mu);
+      l += pe;
+      p[e] = (T)pe;
+    }
+    if (!full) {
+      // slots no row sees - unwritten ones, a refused page's - may hold anything, NaN too
+      bool odd = false;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (vp < 0 || vg + e >= t.kv_end || (!EXACT && 16 * d + m >= dh)) vf[d][e] = (T)0.f;
+          odd |= !(fabsf((float)vf[d][e]) <= 3.4028235e38f);
+        }
+      if (__any(odd)) {
+        // a value that is not finite, in a tile that some rows see only in part: 0 x NaN would reach the rows that do not
+        // see it, so this tile is summed key by key over the rows that do
+        for (int key = 0; key < KT; ++key) {
+          const int pos = base + key, from = (key / E) * 16 + m;
+          float pk = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (key % E == e) pk = __shfl((float)p[e], from, 64);
+          const int pg = pos < t.kv_end ? paged_page(a.ix, t.b, pos) : -1;
+          if (pg < 0) continue;
+          const T* vk = static_cast<const T*>(a.v_pages) + ((((int64_t)pg * a.hkv + kvh) * dh << a.ix.page_log2) + (pos & pmask));
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr) {
+              const int dim = 16 * d + 4 * g + rr;
+              if (pos < vis && (EXACT || dim < dh)) acc[d][rr] = fmaf(pk, to_f32<T>(vk[(int64_t)dim << a.ix.page_log2]), acc[d][rr]);
+            }
+        }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = A::mma(vf[d], p, acc[d]);
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
+  // join the waves: thread (row, part) sums its share of the columns
+  if (g == 0) { ml[w][m][0] = mx; ml[w][m][1] = l; }
+  const int orow = tid / (4 * NW), part = tid % (4 * NW);
+  float M = -INFINITY, L = 0.f, f[NW];
+#pragma unroll
+  for (int p0 = 0; p0 < ND; p0 += NDP) {
+    if (p0) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < NDP; ++d)
+      if (p0 + d < ND) *reinterpret_cast<f32x4*>(&red[w][m][16 * d + 4 * g]) = acc[p0 + d];
+    __syncthreads();
+    if (p0 == 0) {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, ml[i][orow][0]);
+      const float mu = safe_max(M);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        f[i] = fast_exp2(ml[i][orow][0] - mu);
+        L += f[i] * ml[i][orow][1];
+      }
+    }
+    if (orow < t.n_rows) {
+      const int rr = t.row_begin + orow, tok = rr / a.group, hd = kvh * a.group + rr % a.group;
+      const int64_t grow = t.row0 + tok;
+      const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+      for (int c = part * 4; c < NDP * 16; c += 16 * NW) {
+        const int dim = p0 * 16 + c;
+        if (dim >= dh) break;
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&red[i][orow][c]);
+          if (f[i] != 0.f) v += x * f[i];
+        }
+        if (a.splits == 1) {
+          T* op = static_cast<T*>(a.o) + grow * a.ldo + (int64_t)hd * dh + dim;
+          T out[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[j] = from_f32<T>(v[j] * inv);
+          __builtin_memcpy(__builtin_assume_aligned(op, 4 * sizeof(T)), out, sizeof(out));
+        } else {
+          const int64_t wrow = ((int64_t)z * a.ix.tokens + grow) * (a.hkv * a.group) + hd;
+          *reinterpret_cast<f32x4*>(a.ws_o + wrow * DH + dim) = v;
+        }
+      }
+      if (a.splits > 1 && p0 == 0 && part == 0) {
+        const int64_t wrow = ((int64_t)z * a.ix.tokens + grow) * (a.hkv * a.group) + hd;
+        a.ws_ml[2 * wrow] = M;
+        a.ws_ml[2 * wrow + 1] = L;
+      }
+    }
+  }
+}
+
+// joins the splits: one wave a row (token x head)
+template <typename T>
+__global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw, int64_t rows) {
+  const int lane = threadIdx.x & 63, heads = a.hkv * a.group;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t token = row / heads;
+  if (token < a.ix.cu[0] || token >= a.ix.cu[a.ix.batch]) return;      // rows of no sequence stay as they were
+  float M = -INFINITY;
+  for (int z = 0; z < a.splits; ++z) M = fmaxf(M, a.ws_ml[2 * (z * rows + row)]);
+  const float mu = safe_max(M);
+  float L = 0.f;
+  f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int dim = lane * 4;
+  for (int z = 0; z < a.splits; ++z) {
+    const int64_t at = z * rows + row;
+    const float f = fast_exp2(a.ws_ml[2 * at] - mu);
+    if (f == 0.f) continue;
+    L += f * a.ws_ml[2 * at + 1];
+    if (dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + at * ldw + dim) * f;
+  }
+  if (dim >= a.dh) return;
+  const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+  T out[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) out[j] = from_f32<T>(v[j] * inv);
+  T* op = static_cast<T*>(a.o) + token * a.ldo + (row % heads) * a.dh + dim;
+  __builtin_memcpy(__builtin_assume_aligned(op, 4 * sizeof(T)), out, sizeof(out));
+}
+
+static int padded_dh(int64_t dh) {
+  for (int d : {32, 64, 96, 128, 192, 256})
+    if (dh <= d) return d;
+  return 0;
+}
+
+// splits of the keys: enough workgroups for four on every CU, none shorter than 256 keys of the longest possible context
+static int rows_splits(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group) {
+  const int64_t tiles = batch * cdiv64(cdiv64(tokens, batch) * group, 16) * kv_heads;
+  int64_t s = cdiv64(1024, tiles > 0 ? tiles : 1);
+  const int64_t most = cdiv64(wide * page_size, 256);
+  if (s > most) s = most;
+  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+}
+
+extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t q_heads,
+                                                          int64_t kv_heads, int64_t dh, int dtype) {
+  if (tokens <= 0 || batch <= 0 || wide <= 0 || page_size <= 0 || q_heads <= 0 || kv_heads <= 0 || dh <= 0 || dh > 256) return 0;
+  const int s = rows_splits(tokens, batch, wide, page_size, kv_heads, q_heads / kv_heads);
+  return s <= 1 ? 0 : (int64_t)s * tokens * q_heads * (padded_dh(dh) + 2) * 4;
+}
+
+template <typename T> static int attn_launch(PagedAttnArgs a, void* ws, hipStream_t s) {
+  const int pd = padded_dh(a.dh);
+  const int64_t rows = a.ix.tokens * a.hkv * a.group;
+  if (a.splits > 1) {
+    a.ws_o = static_cast<float*>(ws);
+    a.ws_ml = a.ws_o + a.splits * rows * pd;
+  }
+  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, 16, 1), (unsigned)a.hkv, (unsigned)a.splits);
+#define ROWS_CASE(D)                                                                       \
+  case D:                                                                                  \
+    if (a.dh == D) paged_attn_rows<T, D, true, 4><<<grid, 256, 0, s>>>(a);                  \
+    else paged_attn_rows<T, D, false, 4><<<grid, 256, 0, s>>>(a);                           \
+    break;
+  switch (pd) {
+    ROWS_CASE(32) ROWS_CASE(64) ROWS_CASE(96) ROWS_CASE(128) ROWS_CASE(192) ROWS_CASE(256)
+  }
+#undef ROWS_CASE
+  NEURST_CHECK_LAUNCH("paged_attention");
+  if (a.splits > 1) {
+    paged_attn_join<T><<<(unsigned)cdiv64(rows, 4), 256, 0, s>>>(a, pd, rows);
+    NEURST_CHECK_LAUNCH("paged_attention join");
+  }
+  return NEURST_OK;
+}
+
+extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                                      const int32_t* cu_new, const int32_t* ctx_len, int32_t* status, int64_t tokens, int64_t batch,
+                                      int64_t wide, int64_t ld_table, int64_t n_pages, int64_t page_size, int64_t q_heads, int64_t kv_heads,
+                                      int64_t dh, int64_t ldq, int64_t ldo, float scale, int causal, int dtype, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  NEURST_CHECK_ARG(q && k_pages && v_pages && o, "paged_attention: null pointer");
+  PAGED_CHECK_INDEX("paged_attention");
+  NEURST_CHECK_ARG(kv_heads > 0 && kv_heads <= 4096 && q_heads > 0 && q_heads <= 65536 && q_heads % kv_heads == 0,
+                   "paged_attention: q_heads must be a multiple of kv_heads");
+  NEURST_CHECK_ARG(tokens * (q_heads / kv_heads) <= INT32_MAX, "paged_attention: too many rows");
+  NEURST_CHECK_ARG(ldq >= q_heads * dh && ldo >= q_heads * dh, "paged_attention: a row stride is smaller than its heads");
+  NEURST_CHECK_ARG(scale == scale && scale <= 3.4e38f && scale >= -3.4e38f, "paged_attention: scale must be finite");
+  const int64_t es = (int64_t)dtype_size(dtype);
+  const uintptr_t align = (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)(ldq * es) | (uintptr_t)(ldo * es);
+  NEURST_CHECK_ARG(align % 16 == 0, "paged_attention: pointers and row strides must be 16-byte aligned");
+  if (tokens == 0 || batch == 0) return NEURST_OK;
+  PagedAttnArgs a;
+  a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages);
+  a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.o = o; a.status = status;
+  a.ws_o = a.ws_ml = nullptr;
+  a.ldq = ldq; a.ldo = ldo; a.hkv = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.dh = (int)dh; a.causal = causal ? 1 : 0;
+  a.splits = rows_splits(tokens, batch, wide, page_size, kv_heads, a.group);
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  const int64_t need = neurst_paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype);
+  NEURST_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                   "paged_attention: the workspace must hold neurst_paged_attention_workspace_bytes() bytes, 16-byte aligned");
+  return dtype == NEURST_BF16 ? attn_launch<bf16_t>(a, workspace, as_stream(stream)) : attn_launch<float>(a, workspace, as_stream(stream));
+}

@@ -17,7 +17,7 @@ MASK_NONE, MASK_KEYPAD, MASK_CAUSAL = 0, 1, 2
 
 _CTYPES = {
     'int': ctypes.c_int, 'int64_t': ctypes.c_int64, 'int32_t': ctypes.c_int32, 'uint32_t': ctypes.c_uint32,
-    'float': ctypes.c_float, 'void': None,
+    'float': ctypes.c_float, 'double': ctypes.c_double, 'void': None,
 }
 
 

@@ -590,3 +590,245 @@ def gather_rows(src, idx, out=None, row_bytes=None):
     _chk(_C.neurst_gather_rows(_p(src), _p(out), _p(idx), idx.numel(), stride if row_bytes is None else row_bytes, stride, stride, _s()),
          'gather_rows')
     return out
+
+
+# ---- rotary positions ------------------------------------------------------------------------------------------------
+_ROT_LAYOUTS = {'half': 0, 'interleaved': 1}
+
+
+def rotary_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original_length=4096, turns_fast=32.0, turns_slow=1.0, device='cuda'):
+    """-> (freq, mscale): radians per position of the rot_dim / 2 pairs (fp64 tensor on `device`) and the factor on the
+    rotated columns, for `rotary` and `paged_append`.  Pair i turns by base ** (-2 i / rot_dim) a position.  `scaling`
+    stretches a context trained on `original_length` positions by `factor`: None; 'linear': every frequency / factor;
+    'base': base * factor ** (rot_dim / (rot_dim - 2)), the slowest pair / factor and the fastest unchanged; 'parts': pairs
+    that make fewer than turns_slow turns in original_length positions / factor, more than turns_fast unchanged, a line in
+    their turns between, and mscale = 0.1 ln(factor) + 1."""
+    if rot_dim < 2 or rot_dim % 2 or not base > 0 or not factor >= 1.0 or not math.isfinite(base) or not math.isfinite(factor):
+        raise ValueError('rotary: rot_dim must be even and >= 2, base > 0, factor >= 1')
+    if scaling == 'base':
+        if rot_dim < 4:
+            raise ValueError("rotary: scaling 'base' needs rot_dim >= 4")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    f = base ** (-2.0 * np.arange(rot_dim // 2, dtype=np.float64) / rot_dim)
+    mscale = 1.0
+    if scaling == 'linear':
+        f = f / factor
+    elif scaling == 'parts':
+        if not turns_fast > turns_slow or not original_length > 0:
+            raise ValueError('rotary: turns_fast must exceed turns_slow, original_length 0')
+        g = np.clip((original_length * f / (2 * math.pi) - turns_slow) / (turns_fast - turns_slow), 0.0, 1.0)
+        f = f * ((1.0 - g) / factor + g)
+        mscale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, 'none', 'base'):
+        raise ValueError('rotary: unknown scaling {!r}'.format(scaling))
+    return torch.from_numpy(f).to(device), mscale
+
+
+def _want(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+def _on_device(name, dev, *tensors):
+    """launches go to the current device's stream: every tensor has to live there"""
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError('{}: tensors on {} and {}'.format(name, dev, t.device))
+    if dev.type != 'cuda' or dev.index != _cur_dev():
+        raise ValueError('{}: tensors must be on the current GPU, not {}'.format(name, dev))
+
+
+def _heads_view(name, x, what):
+    """[rows, heads, dh] with any row stride, heads and columns packed -> row stride"""
+    _want(x.dim() == 3, '{}: {} must be [rows, heads, dh]'.format(name, what))
+    _want(x.stride(2) == 1 or x.shape[2] == 1, '{}: columns of {} must be contiguous'.format(name, what))
+    _want(x.stride(1) == x.shape[2] or x.shape[1] == 1, '{}: heads of {} must be packed'.format(name, what))
+    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+    _want(ld >= x.shape[1] * x.shape[2], '{}: rows of {} overlap'.format(name, what))
+    return ld
+
+
+def _overlaps(a, b):
+    """whether the memory spans of two tensors meet"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    span = lambda t: (t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size())
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _freq_ok(name, freq, dh):
+    _want(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous(), '{}: freq must be a contiguous fp64 vector'.format(name))
+    _want(1 <= freq.numel() and 2 * freq.numel() <= dh, '{}: freq holds more pairs than a head has columns'.format(name))
+
+
+def rotary(x, freq, positions=None, pos0=0, period=0, layout='half', mscale=1.0, inverse=False, out=None):
+    """The first 2 * len(freq) columns of every head of x [rows, heads, dh] turned by the row's position (neurst_rotary); row r
+    stands at positions[r] (int32), or at pos0 + r, or with a period at pos0 + r % period.  inverse=True turns back: the
+    gradient with respect to x from that of the result.  out: a tensor of x's shape, x itself for in place."""
+    ldx = _heads_view('rotary', x, 'x')
+    dt = dt_of(x)
+    _want(layout in _ROT_LAYOUTS, 'rotary: unknown layout {!r}'.format(layout))
+    _want(math.isfinite(mscale), 'rotary: mscale must be finite')
+    rows, heads, dh = x.shape
+    _freq_ok('rotary', freq, dh)
+    if positions is not None:
+        _want(positions.dtype == torch.int32 and positions.shape == (rows,) and positions.is_contiguous(), 'rotary: positions must be int32 [rows]')
+    if out is None:
+        out = torch.empty((rows, heads, dh), dtype=x.dtype, device=x.device)
+    _want(out.shape == x.shape and out.dtype == x.dtype, 'rotary: out must have the shape and type of x')
+    ldy = _heads_view('rotary', out, 'out')
+    same = out.data_ptr() == x.data_ptr() and ldx == ldy
+    _want(same or not _overlaps(x, out), 'rotary: out overlaps x')
+    _on_device('rotary', x.device, freq, positions, out)
+    _chk(_C.neurst_rotary(_p(x), _p(out), _p(freq), _p(positions), rows, heads, dh, freq.numel(), ldx, ldy, pos0, period,
+                          _ROT_LAYOUTS[layout], int(inverse), mscale, dt, _s()) if rows else 0, 'rotary')
+    return out
+
+
+# ---- paged key / value cache -------------------------------------------------------------------------------------------
+def paged_cache(n_pages, kv_heads, page_size, dh, dtype, device='cuda'):
+    """-> (k_pages [n_pages, kv_heads, page_size, dh], v_pages [n_pages, kv_heads, dh, page_size]), not initialised"""
+    return (torch.empty((n_pages, kv_heads, page_size, dh), dtype=dtype, device=device),
+            torch.empty((n_pages, kv_heads, dh, page_size), dtype=dtype, device=device))
+
+
+def _paged_index(name, k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens):
+    n_pages, kvh, page, dh = k_pages.shape if k_pages.dim() == 4 else (0, 0, 0, 0)
+    _want(n_pages > 0 and v_pages.shape == (n_pages, kvh, dh, page), '{}: pages must be [n, heads, page, dh] and [n, heads, dh, page]'.format(name))
+    _want(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dtype == v_pages.dtype, '{}: pages must be contiguous, of one type'.format(name))
+    B = ctx_len.numel()
+    _want(page_table.dim() == 2 and page_table.shape[0] == B and page_table.shape[1] > 0 and cu_new.shape == (B + 1,) and ctx_len.dim() == 1,
+          '{}: page_table [batch, pages], cu_new [batch + 1], ctx_len [batch]'.format(name))
+    _want(page_table.dtype == cu_new.dtype == ctx_len.dtype == torch.int32, '{}: page_table, cu_new and ctx_len must be int32'.format(name))
+    _want(page_table.stride(1) == 1 or page_table.shape[1] == 1, '{}: rows of page_table must be contiguous'.format(name))
+    _want(cu_new.is_contiguous() and ctx_len.is_contiguous(), '{}: cu_new and ctx_len must be contiguous'.format(name))
+    if status is not None:
+        _want(status.dtype == torch.int32 and status.numel() == 1, '{}: status must be one int32'.format(name))
+    wide = page_table.shape[1]
+    ldt = page_table.stride(0) if B > 1 else wide
+    _want(ldt >= wide or ldt == 0, '{}: rows of page_table overlap'.format(name))
+    return n_pages, kvh, page, dh, B, wide, ldt
+
+
+def paged_append(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q=None, freq=None, layout='half', mscale=1.0, q_out=None, status=None):
+    """New keys and values [tokens, kv_heads, dh] into their pages, the keys and q [tokens, q_heads, dh] turned by position
+    when freq is given (neurst_paged_append; the arrays as there).  Returns the queries (q_out, or a new tensor, whose rows
+    of no sequence are undefined; None without q)."""
+    dt = dt_of(k)
+    ldk, ldv = _heads_view('paged_append', k, 'k'), _heads_view('paged_append', v, 'v')
+    tokens = k.shape[0]
+    n_pages, kvh, page, dh, B, wide, ldt = _paged_index('paged_append', k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens)
+    _want(k.shape == v.shape == (tokens, kvh, dh) and k.dtype == v.dtype == k_pages.dtype, 'paged_append: k and v must be [tokens, kv_heads, dh] of the pages\' type')
+    _want(layout in _ROT_LAYOUTS, 'paged_append: unknown layout {!r}'.format(layout))
+    _want(math.isfinite(mscale), 'paged_append: mscale must be finite')
+    qh = ldq = ldo = 0
+    if freq is not None:
+        _freq_ok('paged_append', freq, dh)
+    if q is not None:
+        ldq, qh = _heads_view('paged_append', q, 'q'), q.shape[1]
+        _want(q.shape == (tokens, qh, dh) and q.dtype == k.dtype, 'paged_append: q must be [tokens, q_heads, dh] of the keys\' type')
+        if q_out is None:
+            q_out = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device)
+        _want(q_out.shape == q.shape and q_out.dtype == q.dtype, 'paged_append: q_out must have the shape and type of q')
+        ldo = _heads_view('paged_append', q_out, 'q_out')
+        _want((q_out.data_ptr() == q.data_ptr() and ldo == ldq) or not _overlaps(q, q_out), 'paged_append: q_out overlaps q')
+        for t in (k, v):
+            _want(q_out.data_ptr() == q.data_ptr() or not _overlaps(t, q_out), 'paged_append: q_out overlaps k or v')
+    else:
+        _want(q_out is None, 'paged_append: q_out without q')
+    _on_device('paged_append', k.device, v, k_pages, v_pages, page_table, cu_new, ctx_len, q, freq, q_out, status)
+    if tokens and B:
+        _chk(_C.neurst_paged_append(_p(k), _p(v), _p(q), _p(k_pages), _p(v_pages), _p(q_out), _p(page_table), _p(cu_new), _p(ctx_len), _p(freq),
+                                    _p(status), tokens, B, wide, ldt, n_pages, page, kvh, qh, dh, ldk, ldv, ldq, ldo,
+                                    0 if freq is None else freq.numel(), _ROT_LAYOUTS[layout], mscale, dt, _s()), 'paged_append')
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, cu_new, ctx_len, scale=None, causal=True, out=None, status=None, workspace=None):
+    """softmax(scale q k^T) v of the new tokens q [tokens, q_heads, dh] over the paged cache (neurst_paged_attention; scale
+    defaults to dh ** -0.5).  out: rows that no sequence owns stay as they are (undefined in a new tensor).  workspace: a
+    uint8 tensor of paged_attention_workspace_bytes(...) kept by the caller for calls that do not overlap; None allocates."""
+    dt = dt_of(q)
+    ldq = _heads_view('paged_attention', q, 'q')
+    tokens, qh, dh_q = q.shape
+    n_pages, kvh, page, dh, B, wide, ldt = _paged_index('paged_attention', k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens)
+    _want(dh_q == dh and q.dtype == k_pages.dtype, 'paged_attention: q must have the pages\' head size and type')
+    _want(qh > 0 and qh % kvh == 0, 'paged_attention: q heads must be a multiple of the key / value heads')
+    scale = dh ** -0.5 if scale is None else float(scale)
+    _want(math.isfinite(scale), 'paged_attention: scale must be finite')
+    if out is None:
+        out = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device)
+    _want(out.shape == q.shape and out.dtype == q.dtype, 'paged_attention: out must have the shape and type of q')
+    ldo = _heads_view('paged_attention', out, 'out')
+    _want(not _overlaps(q, out), 'paged_attention: out overlaps q')
+    _on_device('paged_attention', q.device, k_pages, v_pages, page_table, cu_new, ctx_len, out, status, workspace)
+    if not tokens or not B:
+        return out
+    need = _C.neurst_paged_attention_workspace_bytes(tokens, B, wide, page, qh, kvh, dh, dt)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if _override_stream is not None:
+            workspace.record_stream(_override_stream)
+    _want(not need or workspace.numel() * workspace.element_size() >= need, 'paged_attention: workspace too small')
+    _chk(_C.neurst_paged_attention(_p(q), _p(k_pages), _p(v_pages), _p(out), _p(page_table), _p(cu_new), _p(ctx_len), _p(status), tokens, B, wide,
+                                   ldt, n_pages, page, qh, kvh, dh, ldq, ldo, scale, int(causal), dt, _p(workspace), need, _s()), 'paged_attention')
+    return out
+
+
+def paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype):
+    return int(_C.neurst_paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype))
+
+
+def paged_check(status):
+    """Raises if a kernel found a bad page or length since `status` (int32 [1]) was last zero.  Reads it back: waits."""
+    bits = int(status.cpu()[0])
+    if bits:
+        raise _lib.NeurstLibError('paged cache: ' + ' and '.join(
+            t for b, t in ((1, 'a page id outside the pool'), (2, 'lengths that do not fit')) if bits & b))
+
+
+# ---- sampling ------------------------------------------------------------------------------------------------------------
+def _sample_args(name, logits2d, u, temperature, top_k, top_p, min_p):
+    _want(logits2d.dim() == 2 and (logits2d.stride(1) == 1 or logits2d.shape[1] == 1), '{}: logits must be [rows, V] with contiguous rows'.format(name))
+    R, V = logits2d.shape
+    ld = logits2d.stride(0) if R > 1 else V
+    _want(V > 0 and ld >= V, '{}: rows of logits overlap or are empty'.format(name))
+    _want(u.dtype == torch.float32 and u.shape == (R,) and u.is_contiguous(), '{}: u must be fp32 [rows]'.format(name))
+    rows, scalars = [], []
+    for what, x, dt, default in (('temperature', temperature, torch.float32, 1.0), ('top_k', top_k, torch.int32, 0),
+                                 ('top_p', top_p, torch.float32, 1.0), ('min_p', min_p, torch.float32, 0.0)):
+        if isinstance(x, torch.Tensor):
+            _want(x.dtype == dt and x.shape == (R,) and x.is_contiguous(), '{}: {} per row must be {} [rows]'.format(name, what, dt))
+            rows.append(x)
+            scalars.append(default)
+        else:
+            rows.append(None)
+            scalars.append(min(int(x), 2 ** 31 - 1) if what == 'top_k' else float(x))
+    _on_device(name, logits2d.device, u, *rows)
+    return R, V, ld, [_p(rows[0]), _p(rows[1]), _p(rows[2]), _p(rows[3]), *scalars]
+
+
+def sample(logits2d, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """-> (ids int32 [rows], logp fp32 [rows]): one draw per row of logits from u in [0, 1) (neurst_sample has the rule).
+    Each parameter is a number for all rows or a device tensor with one per row (fp32; top_k int32)."""
+    dt = dt_of(logits2d)
+    R, V, ld, par = _sample_args('sample', logits2d, u, temperature, top_k, top_p, min_p)
+    ids = torch.empty(R, dtype=torch.int32, device=logits2d.device)
+    logp = torch.empty(R, dtype=torch.float32, device=logits2d.device)
+    _chk(_C.neurst_sample(_p(logits2d), _p(u), _p(ids), _p(logp), *par, R, V, ld, dt, _s()) if R else 0, 'sample')
+    return ids, logp
+
+
+def sample_step(logits2d, u, tokens, preds, finished, len_decoded, n_unfinished, scores, step, eos, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The draw of `sample` and the books of a decoding step (neurst_sample_step), as greedy_step keeps them."""
+    dt = dt_of(logits2d)
+    R, V, ld, par = _sample_args('sample_step', logits2d, u, temperature, top_k, top_p, min_p)
+    for t in (tokens, finished, len_decoded):
+        _want(t.dtype == torch.int32 and t.numel() == R and t.is_contiguous(), 'sample_step: tokens, finished and len_decoded must be int32 [rows]')
+    _want(preds.dtype == torch.int32 and preds.dim() == 2 and preds.shape[0] == R and preds.is_contiguous(), 'sample_step: preds must be int32 [rows, steps]')
+    _want(scores.dtype == torch.float32 and scores.shape == (R,) and scores.is_contiguous(), 'sample_step: scores must be fp32 [rows]')
+    _want(n_unfinished.dtype == torch.int32 and n_unfinished.numel() == 1, 'sample_step: n_unfinished must be one int32')
+    _on_device('sample_step', logits2d.device, tokens, preds, finished, len_decoded, n_unfinished, scores)
+    _chk(_C.neurst_sample_step(_p(logits2d), _p(u), _p(tokens), _p(preds), _p(finished), _p(len_decoded), _p(n_unfinished), _p(scores), *par,
+                               R, V, ld, step, preds.shape[1], int(eos), dt, _s()) if R else 0, 'sample_step')
