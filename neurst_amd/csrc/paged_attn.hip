@@ -12,6 +12,13 @@
 // instruction such that a lane's results are eight CONSECUTIVE keys of one query: after exp2 and the rounding to bf16 they
 // are, in place, the operand of O^T = V^T P^T, whose other operand is one 16-byte load from the transposed value pages.  No
 // shared memory and no barrier until the waves join their partial results.
+//
+// paged_attn_tiles: many rows, bf16.  A wave owns 32 rows, a workgroup NW of them; tiles of 64 keys go from the pages to shared
+// memory by direct loads, one tile ahead of the one in use, and all waves read them from there.  The same transposed
+// products with the 32 x 32 x 16 instruction; the key that sits in row r of a 32-key block is chosen again so that a lane's
+// results are runs of eight consecutive keys.
+#include <type_traits>
+
 #include "paged.h"
 
 struct PagedAttnArgs {
@@ -186,26 +193,28 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
           odd |= !(fabsf((float)vf[d][e]) <= 3.4028235e38f);
         }
       if (__any(odd)) {
-        // a value that is not finite, in a tile that some rows see only in part: 0 x NaN would reach the rows that do not
-        // see it, so this tile is summed key by key over the rows that do
-        for (int key = 0; key < KT; ++key) {
-          const int pos = base + key, from = (key / E) * 16 + m;
-          float pk = 0.f;
+        // values that are not finite, in a tile that some rows see only in part (0 x NaN must not reach those that do not):
+        // they are taken out of the product, and added to the rows that see one
+        V seen;
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (key % E == e) pk = __shfl((float)p[e], from, 64);
-          const int pg = pos < t.kv_end ? paged_page(a.ix, t.b, pos) : -1;
-          if (pg < 0) continue;
-          const T* vk = static_cast<const T*>(a.v_pages) + ((((int64_t)pg * a.hkv + kvh) * dh << a.ix.page_log2) + (pos & pmask));
+        for (int e = 0; e < E; ++e) seen[e] = (T)(vp >= 0 && vg + e < vis ? 1.f : 0.f);
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
+          V up, down;
 #pragma unroll
-            for (int rr = 0; rr < 4; ++rr) {
-              const int dim = 16 * d + 4 * g + rr;
-              if (pos < vis && (EXACT || dim < dh)) acc[d][rr] = fmaf(pk, to_f32<T>(vk[(int64_t)dim << a.ix.page_log2]), acc[d][rr]);
-            }
+          for (int e = 0; e < E; ++e) {
+            const float v = (float)vf[d][e];
+            up[e] = (T)(v < INFINITY ? 0.f : 1.f);          // +inf and NaN
+            down[e] = (T)(v > -INFINITY ? 0.f : 1.f);       // -inf and NaN
+            if (!(fabsf(v) <= 3.4028235e38f)) vf[d][e] = (T)0.f;
+          }
+          const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f}, nu = A::mma(up, seen, zero), nd = A::mma(down, seen, zero);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (nu[i] > 0.f) acc[d][i] += INFINITY;
+            if (nd[i] > 0.f) acc[d][i] -= INFINITY;
+          }
         }
-        continue;
       }
     }
 #pragma unroll
@@ -268,6 +277,287 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
   }
 }
 
+// ---- many rows ---------------------------------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+// An image of rows of NC 16-byte chunks: chunk c of row r lies at another place of the row, chosen by r / PER - PER being the
+// rows after which the 256 bytes of all banks come round again - so that the lanes of a read, neighbouring rows with one
+// chunk, spread over the banks.  The direct loads write places in order and fetch the chunk that belongs there.
+template <int NC> struct Image {
+  static constexpr int PER = NC % 16 == 0 ? 1 : NC % 8 == 0 ? 2 : 4;
+  static constexpr bool XOR = (NC & (NC - 1)) == 0;
+  static __device__ __forceinline__ int place(int r, int c) {
+    if constexpr (XOR) return c ^ ((r / PER) & (NC - 1));
+    const int x = c + (r / PER) % NC;
+    return x >= NC ? x - NC : x;
+  }
+  static __device__ __forceinline__ int chunk(int r, int at) {
+    if constexpr (XOR) return at ^ ((r / PER) & (NC - 1));
+    const int x = at - (r / PER) % NC;
+    return x < 0 ? x + NC : x;
+  }
+};
+// key of row r of the key image (32-key blocks), see above: bits 0, 1 stay, 2 -> 3, 3 -> 2, 4 stays
+__device__ __forceinline__ int image_key(int r) { return (r & ~12) | ((r & 4) << 1) | ((r & 8) >> 1); }
+
+__device__ __forceinline__ void load_to_lds(const void* src, char* dst) {      // 16 bytes a lane to dst + 16 * lane
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+template <int DH, bool EXACT, int NW>
+__global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(PagedAttnArgs a) {
+  constexpr int ROWS = 32 * NW, KT = 64, NC = DH / 8, STEPS = DH / 16, ND = DH / 32, IMG = KT * DH * 2;
+  typedef Image<NC> KI;
+  typedef Image<8> VI;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];                 // [2][keys, values]
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.y, z = blockIdx.z;
+  RowTile t;
+  if (!row_tile<ROWS>(a, blockIdx.x, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  const int dh = EXACT ? DH : a.dh;
+  const int page = 1 << a.ix.page_log2, pmask = page - 1;
+  const int row = 32 * w + m;
+  const bool valid = row < t.n_rows;
+  const int r = t.row_begin + (valid ? row : 0), token = r / a.group, head = kvh * a.group + r % a.group;
+  const bf16_t* qp = static_cast<const bf16_t*>(a.q) + (t.row0 + token) * a.ldq + (int64_t)head * dh;
+  const float c_abs = fabsf(a.scale_log2);
+  bf16x8 qf[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int d = 16 * s + 8 * h;
+    u32x4 x = u32x4{0, 0, 0, 0};
+    if (EXACT || d < dh) x = *reinterpret_cast<const u32x4*>(qp + d);
+    if (a.scale_log2 < 0.f) x ^= 0x80008000u;       // the sign of the scale goes to the queries: the maximum is one of s |scale|
+    qf[s] = __builtin_bit_cast(bf16x8, x);
+  }
+  const int vis = a.causal ? (t.kv_end ? t.shift + token + 1 : 0) : t.kv_end;
+  // keys some row of this wave sees, keys all its rows see
+  const int w_rows = t.n_rows - 32 * w;
+  int w_end = 0, w_min = 0;
+  if (w_rows > 0) {
+    w_end = t.kv_end;
+    w_min = t.min_vis;
+    if (a.causal && t.kv_end) {
+      w_end = t.shift + (t.row_begin + 32 * w + (w_rows < 32 ? w_rows : 32) - 1) / a.group + 1;
+      w_min = t.shift + (t.row_begin + 32 * w) / a.group + 1;
+    }
+  }
+  const int nt = (t.kv_end + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits;
+  const int t0 = z * per, t1 = t0 + per < nt ? t0 + per : nt;
+
+  // pages of the four 16-key groups of a tile, in lanes 0..3 of every quad: -1 refused, or beyond the last key
+  auto pages_of = [&](int ti) {
+    const int k = ti * KT + 16 * (lane & 3);
+    const int id = ti < t1 && k < t.kv_end ? paged_page(a.ix, t.b, k) : -1;
+    if (id < 0 && ti < t1 && k < t.kv_end && lane < 4 && w == 0) paged_report(a.status, PAGED_BAD_PAGE);
+    return id;
+  };
+  // A wave's load moves a piece of 64 chunks.  A piece of the key image lies within 16 keys, so within one page: its base is a
+  // scalar and the lanes' offsets are the same for every tile.  A piece of the value image is 8 columns x 64 keys: a lane's
+  // 16-key group is one of two, by the piece's parity.
+  constexpr int NP = (NC + NW - 1) / NW;
+  const char* kpool = static_cast<const char*>(a.k_pages);
+  const char* vpool = static_cast<const char*>(a.v_pages);
+  int koff[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int n = (i * NW + w) * 64 + lane, rr = n / NC, c = KI::chunk(rr, n % NC);
+    koff[i] = ((image_key(rr & 31) & 15 & pmask) * dh + (EXACT || 8 * c < dh ? 8 * c : 0)) * 2;
+  }
+  const int vc = VI::chunk(lane >> 3, lane & 7);           // chunk of an even piece; of an odd one: vc ^ 4
+  const int64_t vrow = (int64_t)(lane >> 3) << (a.ix.page_log2 + 1);
+  auto issue = [&](int ti, int buf, int ids) {
+    char* kimg = smem + buf * 2 * IMG;
+    const int base = ti * KT, slot0 = base & pmask;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int piece = i * NW + w;
+      if (NC % NW == 0 || piece < NC) {
+        const int grp = piece * 4 / NC;                    // the 16-key group
+        int id = __builtin_amdgcn_readlane(ids, grp);
+        id = id < 0 ? 0 : id;
+        const char* src = kpool + (((((int64_t)id * a.hkv + kvh) << a.ix.page_log2) + slot0 + ((16 * grp) & pmask)) * dh) * 2;
+        load_to_lds(src + koff[i], kimg + piece * 1024);
+      }
+    }
+    const char* vsrc[2];
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      const int c = vc ^ (4 * o);
+      int id = __shfl(ids, c >> 1, 64);
+      id = id < 0 ? 0 : id;
+      vsrc[o] = vpool + (((((int64_t)id * a.hkv + kvh) * dh) << a.ix.page_log2) + slot0 + ((8 * c) & pmask)) * 2 + vrow;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int piece = i * NW + w;
+      if ((NC % NW == 0 || piece < NC) && (EXACT || piece * 8 < dh))
+        load_to_lds(vsrc[piece & 1] + ((int64_t)piece << (a.ix.page_log2 + 4)), kimg + IMG + piece * 1024);
+    }
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+  float mx = -INFINITY, l = 0.f;      // maximum in units of log2, sum of this lane's half
+
+  auto compute = [&](int ti, int buf, int ids, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const char* kimg = smem + buf * 2 * IMG;
+    const char* vimg = kimg + IMG;
+    const int base = ti * KT;
+    int mm = m;
+    asm volatile("" : "+v"(mm));                           // image addresses are made here, not kept over the loop
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+      for (int st = 0; st < STEPS; ++st) {
+        const int rr = 32 * b + mm;
+        bf16x8 k = *reinterpret_cast<const bf16x8*>(kimg + (rr * NC + KI::place(rr, 2 * st + h)) * 16);
+        if (!EXACT && 16 * st + 8 * h >= dh) k = bf16x8{};
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[st], s[b], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    unsigned okay = 0xf;
+    if constexpr (MASKED) {
+      okay = (unsigned)(__ballot(ids >= 0) & 0xf);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = 32 * b + 16 * (i >> 3) + 8 * h + (i & 7);
+          if (base + key >= vis || !(okay >> (2 * b + (i >> 3)) & 1)) s[b][i] = -INFINITY;
+        }
+    }
+    float tm = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) tm = fmaxf(tm, s[i >> 4][i & 15]);
+    tm = fmaxf(tm, __shfl_xor(tm, 32, 64)) * c_abs;
+    // the maximum moves only when it has grown by 8 (a factor of 256 in the weights, which fp32 sums and bf16 weights hold
+    // as well as 1): the accumulators are rescaled a few times a row instead of every tile
+    if (__any(tm > mx + 8.f || (mx == -INFINITY && tm > -INFINITY))) {
+      const float mn = fmaxf(mx, tm), al = fast_exp2(mx - safe_max(mn));
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= al;
+      mx = mn;
+    }
+    const float mu = safe_max(mx);
+    bf16x8 p[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float pe = fast_exp2(fmaf(s[i >> 4][i & 15], c_abs, -mu));
+      sum += pe;
+      p[i >> 3][i & 7] = (bf16_t)pe;       // rounded for the second product only, as in the other kernel
+    }
+    l += sum;
+    __builtin_amdgcn_sched_barrier(0);
+    auto values = [&](int ks, int d) {
+      const int rr = 32 * d + mm;
+      return *reinterpret_cast<const bf16x8*>(vimg + (rr * 8 + VI::place(rr, 2 * ks + h)) * 16);
+    };
+    if constexpr (!MASKED) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(ks, d), p[ks], acc[d], 0, 0, 0);
+        if (ks & 1) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const int k0 = base + 16 * ks + 8 * h;
+        const bool ok = okay >> ks & 1;
+        bf16x8 seen;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) seen[e] = (bf16_t)(ok && k0 + e < vis ? 1.f : 0.f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          bf16x8 v = values(ks, d);
+          bool odd = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            // slots no row sees - unwritten ones, a refused page's - may hold anything, NaN too
+            if (!ok || k0 + e >= t.kv_end || (!EXACT && 32 * d + mm >= dh)) v[e] = (bf16_t)0.f;
+            odd |= !(fabsf((float)v[e]) <= 3.4028235e38f);
+          }
+          if (__any(odd)) {      // see the other kernel
+            bf16x8 up, down;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = (float)v[e];
+              up[e] = (bf16_t)(x < INFINITY ? 0.f : 1.f);
+              down[e] = (bf16_t)(x > -INFINITY ? 0.f : 1.f);
+              if (!(fabsf(x) <= 3.4028235e38f)) v[e] = (bf16_t)0.f;
+            }
+            const f32x16 nu = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen, f32x16{}, 0, 0, 0);
+            const f32x16 nd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen, f32x16{}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (nu[i] > 0.f) acc[d][i] += INFINITY;
+              if (nd[i] > 0.f) acc[d][i] -= INFINITY;
+            }
+          }
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[ks], acc[d], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  };
+
+  int ids = pages_of(t0);
+  if (t0 < t1) issue(t0, 0, ids);
+  for (int ti = t0; ti < t1; ++ti) {
+    const int buf = (ti - t0) & 1, next = pages_of(ti + 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of the tile have landed
+    __syncthreads();                                      // everyone's have, and everyone has left the other buffer
+    if (ti + 1 < t1) issue(ti + 1, buf ^ 1, next);
+    const int base = ti * KT;
+    if (base < w_end) {
+      if (base + KT <= w_min && (__ballot(ids >= 0) & 0xf) == 0xf) compute(ti, buf, ids, std::false_type());
+      else compute(ti, buf, ids, std::true_type());
+    }
+    ids = next;
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!valid) return;
+  const int64_t grow = t.row0 + token;
+  if (a.splits == 1) {
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    bf16_t* op = static_cast<bf16_t*>(a.o) + grow * a.ldo + (int64_t)head * dh;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int dim = 32 * d + 2 * i + 4 * h;
+        bf16x4 x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (bf16_t)(acc[d][i + j] * inv);
+        if (EXACT || dim < dh) *reinterpret_cast<bf16x4*>(op + dim) = x;
+      }
+  } else {
+    const int64_t wrow = ((int64_t)z * a.ix.tokens + grow) * (a.hkv * a.group) + head;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int dim = 32 * d + 2 * i + 4 * h;
+        *reinterpret_cast<f32x4*>(a.ws_o + wrow * DH + dim) = f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+      }
+    if (h == 0) {
+      a.ws_ml[2 * wrow] = mx;
+      a.ws_ml[2 * wrow + 1] = l;
+    }
+  }
+}
+
 // joins the splits: one wave a row (token x head)
 template <typename T>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw, int64_t rows) {
@@ -304,39 +594,74 @@ static int padded_dh(int64_t dh) {
   return 0;
 }
 
-// splits of the keys: enough workgroups for four on every CU, none shorter than 256 keys of the longest possible context
-static int rows_splits(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group) {
-  const int64_t tiles = batch * cdiv64(cdiv64(tokens, batch) * group, 16) * kv_heads;
-  int64_t s = cdiv64(1024, tiles > 0 ? tiles : 1);
-  const int64_t most = cdiv64(wide * page_size, 256);
+// What a call launches, from its sizes alone (the lengths are on the device): the kernel by the rows an average sequence
+// brings to a key/value head, and into how many parts the keys are split so that the chip is filled.
+struct AttnPlan { int tiles, waves, splits; };
+static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group, int64_t dh, int dtype,
+                          bool scaled) {
+  AttnPlan p;
+  const int64_t rows = cdiv64(tokens, batch) * group, keys = wide * page_size;
+  p.tiles = dtype == NEURST_BF16 && scaled && rows > 32;
+  p.waves = 4;
+  const int64_t per = p.tiles ? 32 * p.waves : 16, wgs = batch * cdiv64(rows, per) * kv_heads;
+  int64_t s = cdiv64(p.tiles ? 512 : 1024, wgs);
+  const int64_t most = cdiv64(keys, p.tiles ? 1024 : 256);
   if (s > most) s = most;
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  p.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  return p;
 }
 
 extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t q_heads,
                                                           int64_t kv_heads, int64_t dh, int dtype) {
   if (tokens <= 0 || batch <= 0 || wide <= 0 || page_size <= 0 || q_heads <= 0 || kv_heads <= 0 || dh <= 0 || dh > 256) return 0;
-  const int s = rows_splits(tokens, batch, wide, page_size, kv_heads, q_heads / kv_heads);
+  const int64_t group = q_heads / kv_heads;
+  const int a = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, true).splits;
+  const int b = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, false).splits, s = a > b ? a : b;
   return s <= 1 ? 0 : (int64_t)s * tokens * q_heads * (padded_dh(dh) + 2) * 4;
 }
 
-template <typename T> static int attn_launch(PagedAttnArgs a, void* ws, hipStream_t s) {
+template <int DH> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
+  constexpr int NW = 4, LDS = 2 * 2 * 64 * DH * 2;
+  auto kernel = a.dh == DH ? paged_attn_tiles<DH, true, NW> : paged_attn_tiles<DH, false, NW>;
+  if (LDS > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) { neurst_set_error("paged_attention: cannot reserve %d B of LDS: %s", LDS, hipGetErrorString(e)); return NEURST_E_LAUNCH; }
+  }
+  kernel<<<grid, NW * 64, LDS, s>>>(a);
+  return NEURST_OK;
+}
+
+template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, void* ws, hipStream_t s) {
   const int pd = padded_dh(a.dh);
   const int64_t rows = a.ix.tokens * a.hkv * a.group;
   if (a.splits > 1) {
     a.ws_o = static_cast<float*>(ws);
     a.ws_ml = a.ws_o + a.splits * rows * pd;
   }
-  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, 16, 1), (unsigned)a.hkv, (unsigned)a.splits);
+  const int per = plan.tiles ? 32 * plan.waves : 16;
+  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1), (unsigned)a.hkv, (unsigned)a.splits);
+  if (plan.tiles) {
+    if constexpr (sizeof(T) == 2) {
+      switch (pd) {
+        case 32: if (int e = tiles_launch<32>(a, grid, s)) return e; break;
+        case 64: if (int e = tiles_launch<64>(a, grid, s)) return e; break;
+        case 96: if (int e = tiles_launch<96>(a, grid, s)) return e; break;
+        case 128: if (int e = tiles_launch<128>(a, grid, s)) return e; break;
+        case 192: if (int e = tiles_launch<192>(a, grid, s)) return e; break;
+        case 256: if (int e = tiles_launch<256>(a, grid, s)) return e; break;
+      }
+    }
+  } else {
 #define ROWS_CASE(D)                                                                       \
   case D:                                                                                  \
     if (a.dh == D) paged_attn_rows<T, D, true, 4><<<grid, 256, 0, s>>>(a);                  \
     else paged_attn_rows<T, D, false, 4><<<grid, 256, 0, s>>>(a);                           \
     break;
-  switch (pd) {
-    ROWS_CASE(32) ROWS_CASE(64) ROWS_CASE(96) ROWS_CASE(128) ROWS_CASE(192) ROWS_CASE(256)
-  }
+    switch (pd) {
+      ROWS_CASE(32) ROWS_CASE(64) ROWS_CASE(96) ROWS_CASE(128) ROWS_CASE(192) ROWS_CASE(256)
+    }
 #undef ROWS_CASE
+  }
   NEURST_CHECK_LAUNCH("paged_attention");
   if (a.splits > 1) {
     paged_attn_join<T><<<(unsigned)cdiv64(rows, 4), 256, 0, s>>>(a, pd, rows);
@@ -366,10 +691,11 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.o = o; a.status = status;
   a.ws_o = a.ws_ml = nullptr;
   a.ldq = ldq; a.ldo = ldo; a.hkv = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.dh = (int)dh; a.causal = causal ? 1 : 0;
-  a.splits = rows_splits(tokens, batch, wide, page_size, kv_heads, a.group);
+  const AttnPlan plan = attn_plan(tokens, batch, wide, page_size, kv_heads, a.group, dh, dtype, scale != 0.f);
+  a.splits = plan.splits;
   a.scale_log2 = scale * 1.44269504088896340736f;
   const int64_t need = neurst_paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype);
   NEURST_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                    "paged_attention: the workspace must hold neurst_paged_attention_workspace_bytes() bytes, 16-byte aligned");
-  return dtype == NEURST_BF16 ? attn_launch<bf16_t>(a, workspace, as_stream(stream)) : attn_launch<float>(a, workspace, as_stream(stream));
+  return dtype == NEURST_BF16 ? attn_launch<bf16_t>(a, plan, workspace, as_stream(stream)) : attn_launch<float>(a, plan, workspace, as_stream(stream));
 }

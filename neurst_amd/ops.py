@@ -624,28 +624,23 @@ def rotary_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, original
     return torch.from_numpy(f).to(device), mscale
 
 
-def _want(cond, what):
-    if not cond:
-        raise ValueError(what)
+def _row_stride(x, heads, dh):
+    """row stride of x [rows, heads, dh] whose heads and columns are packed, -1 otherwise"""
+    s0, s1, s2 = x.stride()
+    if (s2 != 1 and dh != 1) or (s1 != dh and heads != 1):
+        return -1
+    if x.shape[0] <= 1:
+        return heads * dh
+    return s0 if s0 >= heads * dh else -1
 
 
-def _on_device(name, dev, *tensors):
-    """launches go to the current device's stream: every tensor has to live there"""
+def _here(*tensors):
+    """launches go to the current device's stream: every tensor has to live on that device"""
+    dev = _cur_dev() if tensors[0].is_cuda else -2
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError('{}: tensors on {} and {}'.format(name, dev, t.device))
-    if dev.type != 'cuda' or dev.index != _cur_dev():
-        raise ValueError('{}: tensors must be on the current GPU, not {}'.format(name, dev))
-
-
-def _heads_view(name, x, what):
-    """[rows, heads, dh] with any row stride, heads and columns packed -> row stride"""
-    _want(x.dim() == 3, '{}: {} must be [rows, heads, dh]'.format(name, what))
-    _want(x.stride(2) == 1 or x.shape[2] == 1, '{}: columns of {} must be contiguous'.format(name, what))
-    _want(x.stride(1) == x.shape[2] or x.shape[1] == 1, '{}: heads of {} must be packed'.format(name, what))
-    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
-    _want(ld >= x.shape[1] * x.shape[2], '{}: rows of {} overlap'.format(name, what))
-    return ld
+        if t is not None and t.get_device() != dev:
+            return False
+    return True
 
 
 def _overlaps(a, b):
@@ -657,32 +652,50 @@ def _overlaps(a, b):
     return a0 < b1 and b0 < a1
 
 
-def _freq_ok(name, freq, dh):
-    _want(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous(), '{}: freq must be a contiguous fp64 vector'.format(name))
-    _want(1 <= freq.numel() and 2 * freq.numel() <= dh, '{}: freq holds more pairs than a head has columns'.format(name))
+def _same_rows(a, lda, b, ldb):
+    return a.data_ptr() == b.data_ptr() and lda == ldb
+
+
+def _freq_pairs(freq, dh):
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous():
+        raise ValueError('rotary: freq must be a contiguous fp64 vector')
+    n = freq.numel()
+    if n < 1 or 2 * n > dh:
+        raise ValueError('rotary: freq must hold between one pair and as many as a head has columns for')
+    return n
 
 
 def rotary(x, freq, positions=None, pos0=0, period=0, layout='half', mscale=1.0, inverse=False, out=None):
     """The first 2 * len(freq) columns of every head of x [rows, heads, dh] turned by the row's position (neurst_rotary); row r
     stands at positions[r] (int32), or at pos0 + r, or with a period at pos0 + r % period.  inverse=True turns back: the
     gradient with respect to x from that of the result.  out: a tensor of x's shape, x itself for in place."""
-    ldx = _heads_view('rotary', x, 'x')
     dt = dt_of(x)
-    _want(layout in _ROT_LAYOUTS, 'rotary: unknown layout {!r}'.format(layout))
-    _want(math.isfinite(mscale), 'rotary: mscale must be finite')
+    if x.dim() != 3:
+        raise ValueError('rotary: x must be [rows, heads, dh]')
     rows, heads, dh = x.shape
-    _freq_ok('rotary', freq, dh)
-    if positions is not None:
-        _want(positions.dtype == torch.int32 and positions.shape == (rows,) and positions.is_contiguous(), 'rotary: positions must be int32 [rows]')
+    ldx = _row_stride(x, heads, dh)
+    if ldx < 0:
+        raise ValueError('rotary: heads and columns of x must be packed and its rows apart')
+    if layout not in _ROT_LAYOUTS:
+        raise ValueError('rotary: unknown layout')
+    if not math.isfinite(mscale):
+        raise ValueError('rotary: mscale must be finite')
+    pairs = _freq_pairs(freq, dh)
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous()):
+        raise ValueError('rotary: positions must be int32 [rows]')
     if out is None:
-        out = torch.empty((rows, heads, dh), dtype=x.dtype, device=x.device)
-    _want(out.shape == x.shape and out.dtype == x.dtype, 'rotary: out must have the shape and type of x')
-    ldy = _heads_view('rotary', out, 'out')
-    same = out.data_ptr() == x.data_ptr() and ldx == ldy
-    _want(same or not _overlaps(x, out), 'rotary: out overlaps x')
-    _on_device('rotary', x.device, freq, positions, out)
-    _chk(_C.neurst_rotary(_p(x), _p(out), _p(freq), _p(positions), rows, heads, dh, freq.numel(), ldx, ldy, pos0, period,
-                          _ROT_LAYOUTS[layout], int(inverse), mscale, dt, _s()) if rows else 0, 'rotary')
+        out, ldy = torch.empty((rows, heads, dh), dtype=x.dtype, device=x.device), heads * dh
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError('rotary: out must have the shape and type of x')
+        ldy = _row_stride(out, heads, dh)
+        if ldy < 0 or not (_same_rows(x, ldx, out, ldy) or not _overlaps(x, out)):
+            raise ValueError('rotary: out must be packed like x, and x itself or apart from it')
+    if not _here(x, freq, positions, out):
+        raise ValueError('rotary: every tensor must be on the current GPU')
+    if rows:
+        _chk(_C.neurst_rotary(x.data_ptr(), out.data_ptr(), freq.data_ptr(), _p(positions), rows, heads, dh, pairs, ldx, ldy, pos0, period,
+                              _ROT_LAYOUTS[layout], inverse, mscale, dt, _s()), 'rotary')
     return out
 
 
@@ -693,21 +706,29 @@ def paged_cache(n_pages, kv_heads, page_size, dh, dtype, device='cuda'):
             torch.empty((n_pages, kv_heads, dh, page_size), dtype=dtype, device=device))
 
 
-def _paged_index(name, k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens):
-    n_pages, kvh, page, dh = k_pages.shape if k_pages.dim() == 4 else (0, 0, 0, 0)
-    _want(n_pages > 0 and v_pages.shape == (n_pages, kvh, dh, page), '{}: pages must be [n, heads, page, dh] and [n, heads, dh, page]'.format(name))
-    _want(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.dtype == v_pages.dtype, '{}: pages must be contiguous, of one type'.format(name))
-    B = ctx_len.numel()
-    _want(page_table.dim() == 2 and page_table.shape[0] == B and page_table.shape[1] > 0 and cu_new.shape == (B + 1,) and ctx_len.dim() == 1,
-          '{}: page_table [batch, pages], cu_new [batch + 1], ctx_len [batch]'.format(name))
-    _want(page_table.dtype == cu_new.dtype == ctx_len.dtype == torch.int32, '{}: page_table, cu_new and ctx_len must be int32'.format(name))
-    _want(page_table.stride(1) == 1 or page_table.shape[1] == 1, '{}: rows of page_table must be contiguous'.format(name))
-    _want(cu_new.is_contiguous() and ctx_len.is_contiguous(), '{}: cu_new and ctx_len must be contiguous'.format(name))
-    if status is not None:
-        _want(status.dtype == torch.int32 and status.numel() == 1, '{}: status must be one int32'.format(name))
-    wide = page_table.shape[1]
-    ldt = page_table.stride(0) if B > 1 else wide
-    _want(ldt >= wide or ldt == 0, '{}: rows of page_table overlap'.format(name))
+def _paged_index(k_pages, v_pages, page_table, cu_new, ctx_len, status):
+    """checks what two entry points share -> (n_pages, kv_heads, page_size, dh, batch, wide, ld_table)"""
+    if k_pages.dim() != 4:
+        raise ValueError('paged cache: k_pages must be [n_pages, kv_heads, page_size, dh]')
+    n_pages, kvh, page, dh = k_pages.shape
+    if v_pages.shape != (n_pages, kvh, dh, page) or v_pages.dtype != k_pages.dtype:
+        raise ValueError('paged cache: v_pages must be [n_pages, kv_heads, dh, page_size] of the type of k_pages')
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError('paged cache: pages must be contiguous')
+    if page_table.dim() != 2 or ctx_len.dim() != 1:
+        raise ValueError('paged cache: page_table must be [batch, pages], ctx_len [batch]')
+    B, wide = page_table.shape
+    if ctx_len.shape[0] != B or cu_new.shape != (B + 1,) or wide == 0:
+        raise ValueError('paged cache: page_table [batch, pages], cu_new [batch + 1] and ctx_len [batch] do not fit')
+    if page_table.dtype != torch.int32 or cu_new.dtype != torch.int32 or ctx_len.dtype != torch.int32:
+        raise ValueError('paged cache: page_table, cu_new and ctx_len must be int32')
+    ldt, s1 = page_table.stride()
+    if B <= 1:
+        ldt = wide
+    if (s1 != 1 and wide != 1) or (ldt < wide and ldt != 0) or not (cu_new.is_contiguous() and ctx_len.is_contiguous()):
+        raise ValueError('paged cache: rows of page_table, cu_new and ctx_len must be contiguous')
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError('paged cache: status must be one int32')
     return n_pages, kvh, page, dh, B, wide, ldt
 
 
@@ -716,32 +737,40 @@ def paged_append(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q=None, fr
     when freq is given (neurst_paged_append; the arrays as there).  Returns the queries (q_out, or a new tensor, whose rows
     of no sequence are undefined; None without q)."""
     dt = dt_of(k)
-    ldk, ldv = _heads_view('paged_append', k, 'k'), _heads_view('paged_append', v, 'v')
+    n_pages, kvh, page, dh, B, wide, ldt = _paged_index(k_pages, v_pages, page_table, cu_new, ctx_len, status)
     tokens = k.shape[0]
-    n_pages, kvh, page, dh, B, wide, ldt = _paged_index('paged_append', k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens)
-    _want(k.shape == v.shape == (tokens, kvh, dh) and k.dtype == v.dtype == k_pages.dtype, 'paged_append: k and v must be [tokens, kv_heads, dh] of the pages\' type')
-    _want(layout in _ROT_LAYOUTS, 'paged_append: unknown layout {!r}'.format(layout))
-    _want(math.isfinite(mscale), 'paged_append: mscale must be finite')
+    if k.shape != (tokens, kvh, dh) or v.shape != k.shape or k.dtype != k_pages.dtype or v.dtype != k.dtype:
+        raise ValueError('paged_append: k and v must be [tokens, kv_heads, dh] of the type of the pages')
+    ldk, ldv = _row_stride(k, kvh, dh), _row_stride(v, kvh, dh)
+    if ldk < 0 or ldv < 0:
+        raise ValueError('paged_append: heads and columns of k and v must be packed and their rows apart')
+    if layout not in _ROT_LAYOUTS or not math.isfinite(mscale):
+        raise ValueError('paged_append: unknown layout, or mscale is not finite')
+    pairs = 0 if freq is None else _freq_pairs(freq, dh)
     qh = ldq = ldo = 0
-    if freq is not None:
-        _freq_ok('paged_append', freq, dh)
     if q is not None:
-        ldq, qh = _heads_view('paged_append', q, 'q'), q.shape[1]
-        _want(q.shape == (tokens, qh, dh) and q.dtype == k.dtype, 'paged_append: q must be [tokens, q_heads, dh] of the keys\' type')
+        qh = q.shape[1]
+        if q.shape != (tokens, qh, dh) or q.dtype != k.dtype:
+            raise ValueError('paged_append: q must be [tokens, q_heads, dh] of the type of the keys')
+        ldq = _row_stride(q, qh, dh)
         if q_out is None:
-            q_out = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device)
-        _want(q_out.shape == q.shape and q_out.dtype == q.dtype, 'paged_append: q_out must have the shape and type of q')
-        ldo = _heads_view('paged_append', q_out, 'q_out')
-        _want((q_out.data_ptr() == q.data_ptr() and ldo == ldq) or not _overlaps(q, q_out), 'paged_append: q_out overlaps q')
-        for t in (k, v):
-            _want(q_out.data_ptr() == q.data_ptr() or not _overlaps(t, q_out), 'paged_append: q_out overlaps k or v')
-    else:
-        _want(q_out is None, 'paged_append: q_out without q')
-    _on_device('paged_append', k.device, v, k_pages, v_pages, page_table, cu_new, ctx_len, q, freq, q_out, status)
+            q_out, ldo = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device), qh * dh
+        else:
+            if q_out.shape != q.shape or q_out.dtype != q.dtype:
+                raise ValueError('paged_append: q_out must have the shape and type of q')
+            ldo = _row_stride(q_out, qh, dh)
+            if not _same_rows(q, ldq, q_out, ldo) and (_overlaps(q, q_out) or _overlaps(k, q_out) or _overlaps(v, q_out)):
+                raise ValueError('paged_append: q_out must be q itself or apart from q, k and v')
+        if ldq < 0 or ldo < 0:
+            raise ValueError('paged_append: heads and columns of q and q_out must be packed and their rows apart')
+    elif q_out is not None:
+        raise ValueError('paged_append: q_out without q')
+    if not _here(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q, freq, q_out, status):
+        raise ValueError('paged_append: every tensor must be on the current GPU')
     if tokens and B:
-        _chk(_C.neurst_paged_append(_p(k), _p(v), _p(q), _p(k_pages), _p(v_pages), _p(q_out), _p(page_table), _p(cu_new), _p(ctx_len), _p(freq),
-                                    _p(status), tokens, B, wide, ldt, n_pages, page, kvh, qh, dh, ldk, ldv, ldq, ldo,
-                                    0 if freq is None else freq.numel(), _ROT_LAYOUTS[layout], mscale, dt, _s()), 'paged_append')
+        _chk(_C.neurst_paged_append(k.data_ptr(), v.data_ptr(), _p(q), k_pages.data_ptr(), v_pages.data_ptr(), _p(q_out), page_table.data_ptr(),
+                                    cu_new.data_ptr(), ctx_len.data_ptr(), _p(freq), _p(status), tokens, B, wide, ldt, n_pages, page, kvh, qh, dh,
+                                    ldk, ldv, ldq, ldo, pairs, _ROT_LAYOUTS[layout], mscale, dt, _s()), 'paged_append')
     return q_out
 
 
@@ -750,29 +779,41 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_new, ctx_len, scale=None
     defaults to dh ** -0.5).  out: rows that no sequence owns stay as they are (undefined in a new tensor).  workspace: a
     uint8 tensor of paged_attention_workspace_bytes(...) kept by the caller for calls that do not overlap; None allocates."""
     dt = dt_of(q)
-    ldq = _heads_view('paged_attention', q, 'q')
-    tokens, qh, dh_q = q.shape
-    n_pages, kvh, page, dh, B, wide, ldt = _paged_index('paged_attention', k_pages, v_pages, page_table, cu_new, ctx_len, status, tokens)
-    _want(dh_q == dh and q.dtype == k_pages.dtype, 'paged_attention: q must have the pages\' head size and type')
-    _want(qh > 0 and qh % kvh == 0, 'paged_attention: q heads must be a multiple of the key / value heads')
+    n_pages, kvh, page, dh, B, wide, ldt = _paged_index(k_pages, v_pages, page_table, cu_new, ctx_len, status)
+    if q.dim() != 3 or q.shape[2] != dh or q.dtype != k_pages.dtype:
+        raise ValueError('paged_attention: q must be [tokens, q_heads, dh] of the type of the pages')
+    tokens, qh = q.shape[0], q.shape[1]
+    if qh == 0 or qh % kvh:
+        raise ValueError('paged_attention: q heads must be a multiple of the key / value heads')
+    ldq = _row_stride(q, qh, dh)
+    if ldq < 0:
+        raise ValueError('paged_attention: heads and columns of q must be packed and its rows apart')
     scale = dh ** -0.5 if scale is None else float(scale)
-    _want(math.isfinite(scale), 'paged_attention: scale must be finite')
+    if not math.isfinite(scale):
+        raise ValueError('paged_attention: scale must be finite')
     if out is None:
-        out = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device)
-    _want(out.shape == q.shape and out.dtype == q.dtype, 'paged_attention: out must have the shape and type of q')
-    ldo = _heads_view('paged_attention', out, 'out')
-    _want(not _overlaps(q, out), 'paged_attention: out overlaps q')
-    _on_device('paged_attention', q.device, k_pages, v_pages, page_table, cu_new, ctx_len, out, status, workspace)
+        out, ldo = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device), qh * dh
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError('paged_attention: out must have the shape and type of q')
+        ldo = _row_stride(out, qh, dh)
+        if ldo < 0 or _overlaps(q, out):
+            raise ValueError('paged_attention: out must be packed like q and apart from it')
+    if not _here(q, k_pages, v_pages, page_table, cu_new, ctx_len, out, status, workspace):
+        raise ValueError('paged_attention: every tensor must be on the current GPU')
     if not tokens or not B:
         return out
     need = _C.neurst_paged_attention_workspace_bytes(tokens, B, wide, page, qh, kvh, dh, dt)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        if _override_stream is not None:
-            workspace.record_stream(_override_stream)
-    _want(not need or workspace.numel() * workspace.element_size() >= need, 'paged_attention: workspace too small')
-    _chk(_C.neurst_paged_attention(_p(q), _p(k_pages), _p(v_pages), _p(out), _p(page_table), _p(cu_new), _p(ctx_len), _p(status), tokens, B, wide,
-                                   ldt, n_pages, page, qh, kvh, dh, ldq, ldo, scale, int(causal), dt, _p(workspace), need, _s()), 'paged_attention')
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            if _override_stream is not None:
+                workspace.record_stream(_override_stream)
+        elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
+            raise ValueError('paged_attention: workspace must be contiguous, of paged_attention_workspace_bytes() bytes')
+    _chk(_C.neurst_paged_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(), cu_new.data_ptr(),
+                                   ctx_len.data_ptr(), _p(status), tokens, B, wide, ldt, n_pages, page, qh, kvh, dh, ldq, ldo, scale, causal, dt,
+                                   _p(workspace), need, _s()), 'paged_attention')
     return out
 
 
@@ -789,46 +830,61 @@ def paged_check(status):
 
 
 # ---- sampling ------------------------------------------------------------------------------------------------------------
-def _sample_args(name, logits2d, u, temperature, top_k, top_p, min_p):
-    _want(logits2d.dim() == 2 and (logits2d.stride(1) == 1 or logits2d.shape[1] == 1), '{}: logits must be [rows, V] with contiguous rows'.format(name))
+_SAMPLE_ROWS = (('temperature', torch.float32, 1.0), ('top_k', torch.int32, 0), ('top_p', torch.float32, 1.0), ('min_p', torch.float32, 0.0))
+
+
+def _sample_args(logits2d, u, values):
+    """-> rows, V, row stride, and the parameters as the C entries take them: four pointers, four numbers"""
+    if logits2d.dim() != 2:
+        raise ValueError('sample: logits must be [rows, V]')
     R, V = logits2d.shape
-    ld = logits2d.stride(0) if R > 1 else V
-    _want(V > 0 and ld >= V, '{}: rows of logits overlap or are empty'.format(name))
-    _want(u.dtype == torch.float32 and u.shape == (R,) and u.is_contiguous(), '{}: u must be fp32 [rows]'.format(name))
-    rows, scalars = [], []
-    for what, x, dt, default in (('temperature', temperature, torch.float32, 1.0), ('top_k', top_k, torch.int32, 0),
-                                 ('top_p', top_p, torch.float32, 1.0), ('min_p', min_p, torch.float32, 0.0)):
+    ld, s1 = logits2d.stride()
+    if R <= 1:
+        ld = V
+    if V == 0 or ld < V or (s1 != 1 and V != 1):
+        raise ValueError('sample: rows of logits must be contiguous, apart and not empty')
+    if u.dtype != torch.float32 or u.shape != (R,) or not u.is_contiguous():
+        raise ValueError('sample: u must be fp32 [rows]')
+    if not _here(logits2d, u):
+        raise ValueError('sample: every tensor must be on the current GPU')
+    pointers, numbers = [0, 0, 0, 0], list(values)
+    for i, x in enumerate(values):
         if isinstance(x, torch.Tensor):
-            _want(x.dtype == dt and x.shape == (R,) and x.is_contiguous(), '{}: {} per row must be {} [rows]'.format(name, what, dt))
-            rows.append(x)
-            scalars.append(default)
-        else:
-            rows.append(None)
-            scalars.append(min(int(x), 2 ** 31 - 1) if what == 'top_k' else float(x))
-    _on_device(name, logits2d.device, u, *rows)
-    return R, V, ld, [_p(rows[0]), _p(rows[1]), _p(rows[2]), _p(rows[3]), *scalars]
+            what, dt, default = _SAMPLE_ROWS[i]
+            if x.dtype != dt or x.shape != (R,) or not x.is_contiguous() or not _here(logits2d, x):
+                raise ValueError('sample: {} per row must be {} [rows] on the current GPU'.format(what, dt))
+            pointers[i], numbers[i] = x.data_ptr(), default
+    numbers[1] = min(int(numbers[1]), 0x7fffffff)
+    return R, V, ld, pointers + numbers
 
 
 def sample(logits2d, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """-> (ids int32 [rows], logp fp32 [rows]): one draw per row of logits from u in [0, 1) (neurst_sample has the rule).
     Each parameter is a number for all rows or a device tensor with one per row (fp32; top_k int32)."""
     dt = dt_of(logits2d)
-    R, V, ld, par = _sample_args('sample', logits2d, u, temperature, top_k, top_p, min_p)
+    R, V, ld, par = _sample_args(logits2d, u, (temperature, top_k, top_p, min_p))
     ids = torch.empty(R, dtype=torch.int32, device=logits2d.device)
     logp = torch.empty(R, dtype=torch.float32, device=logits2d.device)
-    _chk(_C.neurst_sample(_p(logits2d), _p(u), _p(ids), _p(logp), *par, R, V, ld, dt, _s()) if R else 0, 'sample')
+    if R:
+        _chk(_C.neurst_sample(logits2d.data_ptr(), u.data_ptr(), ids.data_ptr(), logp.data_ptr(), *par, R, V, ld, dt, _s()), 'sample')
     return ids, logp
 
 
 def sample_step(logits2d, u, tokens, preds, finished, len_decoded, n_unfinished, scores, step, eos, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """The draw of `sample` and the books of a decoding step (neurst_sample_step), as greedy_step keeps them."""
     dt = dt_of(logits2d)
-    R, V, ld, par = _sample_args('sample_step', logits2d, u, temperature, top_k, top_p, min_p)
+    R, V, ld, par = _sample_args(logits2d, u, (temperature, top_k, top_p, min_p))
     for t in (tokens, finished, len_decoded):
-        _want(t.dtype == torch.int32 and t.numel() == R and t.is_contiguous(), 'sample_step: tokens, finished and len_decoded must be int32 [rows]')
-    _want(preds.dtype == torch.int32 and preds.dim() == 2 and preds.shape[0] == R and preds.is_contiguous(), 'sample_step: preds must be int32 [rows, steps]')
-    _want(scores.dtype == torch.float32 and scores.shape == (R,) and scores.is_contiguous(), 'sample_step: scores must be fp32 [rows]')
-    _want(n_unfinished.dtype == torch.int32 and n_unfinished.numel() == 1, 'sample_step: n_unfinished must be one int32')
-    _on_device('sample_step', logits2d.device, tokens, preds, finished, len_decoded, n_unfinished, scores)
-    _chk(_C.neurst_sample_step(_p(logits2d), _p(u), _p(tokens), _p(preds), _p(finished), _p(len_decoded), _p(n_unfinished), _p(scores), *par,
-                               R, V, ld, step, preds.shape[1], int(eos), dt, _s()) if R else 0, 'sample_step')
+        if t.dtype != torch.int32 or t.numel() != R or not t.is_contiguous():
+            raise ValueError('sample_step: tokens, finished and len_decoded must be int32 [rows]')
+    if preds.dtype != torch.int32 or preds.dim() != 2 or preds.shape[0] != R or not preds.is_contiguous():
+        raise ValueError('sample_step: preds must be int32 [rows, steps]')
+    if scores.dtype != torch.float32 or scores.shape != (R,) or not scores.is_contiguous():
+        raise ValueError('sample_step: scores must be fp32 [rows]')
+    if n_unfinished.dtype != torch.int32 or n_unfinished.numel() != 1:
+        raise ValueError('sample_step: n_unfinished must be one int32')
+    if not _here(logits2d, tokens, preds, finished, len_decoded, n_unfinished, scores):
+        raise ValueError('sample_step: every tensor must be on the current GPU')
+    if R:
+        _chk(_C.neurst_sample_step(logits2d.data_ptr(), u.data_ptr(), tokens.data_ptr(), preds.data_ptr(), finished.data_ptr(), len_decoded.data_ptr(),
+                                   n_unfinished.data_ptr(), scores.data_ptr(), *par, R, V, ld, step, preds.shape[1], int(eos), dt, _s()), 'sample_step')
