@@ -25,10 +25,11 @@ struct PagedAttnArgs {
   PagedIndex ix;
   const void *q, *k_pages, *v_pages;
   void* o;
-  float *ws_o, *ws_ml;      // splits > 1: partial results [split][row][dh padded], [split][row][2]
+  float *ws_o, *ws_ml;      // parts > 1: partial results [part][row][dh padded], [part][row][2]
   int32_t* status;
   int64_t ldq, ldo;
-  int hkv, group, dh, causal, splits;
+  int hkv, group, dh, causal;
+  int parts, part_keys;     // the keys in parts of part_keys, one workgroup each
   float scale_log2;         // scale * log2(e): exp(x) = exp2(x log2(e))
 };
 
@@ -79,8 +80,15 @@ template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs
   return true;
 }
 
+// a part in which a row sees no key: no sum, and no partial result to read
+__device__ __forceinline__ void part_nothing(const PagedAttnArgs& a, const RowTile& t, int kvh, int z, int row) {
+  const int64_t wrow = ((int64_t)z * a.ix.tokens + t.row0 + row / a.group) * (a.hkv * a.group) + kvh * a.group + row % a.group;
+  a.ws_ml[2 * wrow] = -INFINITY;
+  a.ws_ml[2 * wrow + 1] = 0.f;
+}
+
 template <typename T, int DH, bool EXACT, int NW>
-__global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
+__global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 128 ? 2 : 1) paged_attn_rows(PagedAttnArgs a) {
   typedef PagedMma<T> A;
   typedef typename A::V V;
   constexpr int E = A::E, KT = A::KT, NSUB = A::NSUB, KC = DH / (4 * E), ND = DH / 16;
@@ -107,38 +115,61 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
       for (int e = 0; e < E; ++e) qf[c][e] = (T)0.f;
   }
   const int vis = a.causal ? (t.kv_end ? t.shift + token + 1 : 0) : t.kv_end;
-  // this split's tiles
-  const int nt = (t.kv_end + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits;
+  // this part's tiles
+  const int nt = (t.kv_end + KT - 1) / KT, per = a.part_keys / KT;
   const int t0 = z * per, t1 = t0 + per < nt ? t0 + per : nt;
+  if (t0 >= t1 && a.parts > 1) {
+    if (tid < t.n_rows) part_nothing(a, t, kvh, z, t.row_begin + tid);
+    return;
+  }
 
   f32x4 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   float mx = -INFINITY, l = 0.f;
-  for (int ti = t0 + w; ti < t1; ti += NW) {
-    const int base = ti * KT;
-    // pages of the E-key groups this lane reads: keys of group m >> 2 for the first product, of group g for the second
-    const int kg = base + E * (m >> 2), vg = base + E * g;
-    const int kp = kg < t.kv_end ? paged_page(a.ix, t.b, kg) : -1;
-    const int vp = vg < t.kv_end ? paged_page(a.ix, t.b, vg) : -1;
-    if (vp < 0 && vg < t.kv_end) paged_report(a.status, PAGED_BAD_PAGE);
-    const bool full = base + KT <= t.min_vis && __all(vp >= 0);
-    const T* kb = static_cast<const T*>(a.k_pages) +
-                  (((((int64_t)(kp < 0 ? 0 : kp) * a.hkv + kvh) << a.ix.page_log2) + (kg & pmask) + (m & 3)) * dh);
-    const T* vb = static_cast<const T*>(a.v_pages) + ((((int64_t)(vp < 0 ? 0 : vp) * a.hkv + kvh) * dh << a.ix.page_log2) + (vg & pmask));
-    V kf[NSUB][KC], vf[ND];
+  // Pages of the E-key groups this lane reads of a tile: keys of group m >> 2 for the first product, of group g for the
+  // second; -1 refused, or beyond the last key.
+  auto page_at = [&](int k) { return k < t.kv_end ? paged_page(a.ix, t.b, k) : -1; };
+  auto load_k = [&](int ti, int id, V (&kf)[NSUB][KC]) {
+    const int slot = ((ti * KT + E * (m >> 2)) & pmask) + (m & 3);
+    const T* kb = static_cast<const T*>(a.k_pages) + ((((int64_t)(id < 0 ? 0 : id) * a.hkv + kvh) << a.ix.page_log2) + slot) * dh;
 #pragma unroll
     for (int s = 0; s < NSUB; ++s)
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const int d = c * 4 * E + E * g;
-        kf[s][c] = *reinterpret_cast<const V*>(kb + (int64_t)4 * s * dh + (EXACT || d < dh ? d : 0));
+        kf[s][c] = *reinterpret_cast<const V*>(kb + 4 * s * dh + (EXACT || d < dh ? d : 0));
       }
+  };
+  auto load_v = [&](int ti, int id, V (&vf)[ND]) {
+    const T* vb = static_cast<const T*>(a.v_pages) + ((((int64_t)(id < 0 ? 0 : id) * a.hkv + kvh) * dh << a.ix.page_log2) + ((ti * KT + E * g) & pmask));
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       const int dim = 16 * d + m;
       vf[d] = *reinterpret_cast<const V*>(vb + ((int64_t)(EXACT || dim < dh ? dim : 0) << a.ix.page_log2));
     }
+  };
+  // The loads of a wave's next tile go out as soon as the products have taken the registers of this one - the keys' after the
+  // first, the values' after the second - and its pages are looked up one tile earlier still, so that the memory always has
+  // most of a tile per wave to work on.
+  V kf[NSUB][KC], vf[ND];
+  int vp = -1, kp1 = -1, vp1 = -1;
+  if (t0 + w < t1) {
+    const int ti = t0 + w;
+    const int kp = page_at(ti * KT + E * (m >> 2));
+    vp = page_at(ti * KT + E * g);
+    if (ti + NW < t1) {
+      kp1 = page_at((ti + NW) * KT + E * (m >> 2));
+      vp1 = page_at((ti + NW) * KT + E * g);
+    }
+    load_k(ti, kp, kf);
+    load_v(ti, vp, vf);
+  }
+  for (int ti = t0 + w; ti < t1; ti += NW) {
+    const int base = ti * KT, vg = base + E * g;
+    const bool more = ti + NW < t1;
+    if (vp < 0 && vg < t.kv_end) paged_report(a.status, PAGED_BAD_PAGE);
+    const bool full = base + KT <= t.min_vis && __all(vp >= 0);
     f32x4 sc[NSUB];
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
@@ -152,6 +183,15 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
         sc[s] = A::mma(k, qf[c], sc[s]);
       }
     }
+    int kp2 = -1, vp2 = -1;
+    if (more) {
+      load_k(ti + NW, kp1, kf);
+      if (ti + 2 * NW < t1) {
+        kp2 = page_at((ti + 2 * NW) * KT + E * (m >> 2));
+        vp2 = page_at((ti + 2 * NW) * KT + E * g);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     float x[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = sc[e >> 2][e & 3] * a.scale_log2;     // keys vg + e of query m
@@ -214,11 +254,17 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
             if (nu[i] > 0.f) acc[d][i] += INFINITY;
             if (nd[i] > 0.f) acc[d][i] -= INFINITY;
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = A::mma(vf[d], p, acc[d]);
+    if (more) load_v(ti + NW, vp1, vf);
+    __builtin_amdgcn_sched_barrier(0);
+    vp = vp1;
+    kp1 = kp2;
+    vp1 = vp2;
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -257,7 +303,7 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(&red[i][orow][c]);
           if (f[i] != 0.f) v += x * f[i];
         }
-        if (a.splits == 1) {
+        if (a.parts == 1) {
           T* op = static_cast<T*>(a.o) + grow * a.ldo + (int64_t)hd * dh + dim;
           T out[4];
 #pragma unroll
@@ -268,7 +314,7 @@ __global__ void __launch_bounds__(NW * 64) paged_attn_rows(PagedAttnArgs a) {
           *reinterpret_cast<f32x4*>(a.ws_o + wrow * DH + dim) = v;
         }
       }
-      if (a.splits > 1 && p0 == 0 && part == 0) {
+      if (a.parts > 1 && p0 == 0 && part == 0) {
         const int64_t wrow = ((int64_t)z * a.ix.tokens + grow) * (a.hkv * a.group) + hd;
         a.ws_ml[2 * wrow] = M;
         a.ws_ml[2 * wrow + 1] = L;
@@ -342,8 +388,12 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
       w_min = t.shift + (t.row_begin + 32 * w) / a.group + 1;
     }
   }
-  const int nt = (t.kv_end + KT - 1) / KT, per = (nt + a.splits - 1) / a.splits;
+  const int nt = (t.kv_end + KT - 1) / KT, per = a.part_keys / KT;
   const int t0 = z * per, t1 = t0 + per < nt ? t0 + per : nt;
+  if (t0 >= t1 && a.parts > 1) {
+    if (valid && h == 0) part_nothing(a, t, kvh, z, r);
+    return;
+  }
 
   // pages of the four 16-key groups of a tile, in lanes 0..3 of every quad: -1 refused, or beyond the last key
   auto pages_of = [&](int ti) {
@@ -529,7 +579,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
   l += __shfl_xor(l, 32, 64);
   if (!valid) return;
   const int64_t grow = t.row0 + token;
-  if (a.splits == 1) {
+  if (a.parts == 1) {
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     bf16_t* op = static_cast<bf16_t*>(a.o) + grow * a.ldo + (int64_t)head * dh;
 #pragma unroll
@@ -558,7 +608,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
   }
 }
 
-// joins the splits: one wave a row (token x head)
+// joins the parts: one wave a row (token x head)
 template <typename T>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw, int64_t rows) {
   const int lane = threadIdx.x & 63, heads = a.hkv * a.group;
@@ -566,18 +616,19 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw,
   if (row >= rows) return;
   const int64_t token = row / heads;
   if (token < a.ix.cu[0] || token >= a.ix.cu[a.ix.batch]) return;      // rows of no sequence stay as they were
-  float M = -INFINITY;
-  for (int z = 0; z < a.splits; ++z) M = fmaxf(M, a.ws_ml[2 * (z * rows + row)]);
-  const float mu = safe_max(M);
-  float L = 0.f;
+  // lane z holds part z's maximum and sum (at most 64 parts), and what its partial result counts
+  float pm = -INFINITY, pl = 0.f;
+  if (lane < a.parts) {
+    const int64_t at = 2 * (lane * rows + row);
+    pm = a.ws_ml[at];
+    pl = a.ws_ml[at + 1];
+  }
+  const float M = wave_max(pm), f = fast_exp2(pm - safe_max(M)), L = wave_sum(f == 0.f ? 0.f : f * pl);
   f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
   const int dim = lane * 4;
-  for (int z = 0; z < a.splits; ++z) {
-    const int64_t at = z * rows + row;
-    const float f = fast_exp2(a.ws_ml[2 * at] - mu);
-    if (f == 0.f) continue;
-    L += f * a.ws_ml[2 * at + 1];
-    if (dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + at * ldw + dim) * f;
+  for (int z = 0; z < a.parts; ++z) {
+    const float fz = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), z));
+    if (fz != 0.f && dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + (z * rows + row) * ldw + dim) * fz;
   }
   if (dim >= a.dh) return;
   const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
@@ -596,18 +647,19 @@ static int padded_dh(int64_t dh) {
 
 // What a call launches, from its sizes alone (the lengths are on the device): the kernel by the rows an average sequence
 // brings to a key/value head, and into how many parts the keys are split so that the chip is filled.
-struct AttnPlan { int tiles, waves, splits; };
+struct AttnPlan { int tiles, parts, part_keys; };
 static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group, int64_t dh, int dtype,
                           bool scaled) {
   AttnPlan p;
   const int64_t rows = cdiv64(tokens, batch) * group, keys = wide * page_size;
   p.tiles = dtype == NEURST_BF16 && scaled && rows > 32;
-  p.waves = 4;
-  const int64_t per = p.tiles ? 32 * p.waves : 16, wgs = batch * cdiv64(rows, per) * kv_heads;
-  int64_t s = cdiv64(p.tiles ? 512 : 1024, wgs);
-  const int64_t most = cdiv64(keys, p.tiles ? 1024 : 256);
-  if (s > most) s = most;
-  p.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+  const int64_t wgs = batch * cdiv64(rows, p.tiles ? 128 : 16) * kv_heads;
+  // parts of equal length, not of equal number a sequence: the workgroups of a ragged batch then take equally long
+  const int64_t least = p.tiles ? 1024 : 512, want = p.tiles ? 512 : 4096;
+  int64_t part = cdiv64(cdiv64(keys * wgs, want), least) * least;
+  if (part * 64 < keys) part = cdiv64(cdiv64(keys, 64), least) * least;
+  p.part_keys = (int)(part < keys ? part : cdiv64(keys, 64) * 64);
+  p.parts = (int)cdiv64(keys, p.part_keys);
   return p;
 }
 
@@ -615,8 +667,8 @@ extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_
                                                           int64_t kv_heads, int64_t dh, int dtype) {
   if (tokens <= 0 || batch <= 0 || wide <= 0 || page_size <= 0 || q_heads <= 0 || kv_heads <= 0 || dh <= 0 || dh > 256) return 0;
   const int64_t group = q_heads / kv_heads;
-  const int a = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, true).splits;
-  const int b = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, false).splits, s = a > b ? a : b;
+  const int a = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, true).parts;
+  const int b = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, false).parts, s = a > b ? a : b;
   return s <= 1 ? 0 : (int64_t)s * tokens * q_heads * (padded_dh(dh) + 2) * 4;
 }
 
@@ -634,12 +686,12 @@ template <int DH> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hip
 template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, void* ws, hipStream_t s) {
   const int pd = padded_dh(a.dh);
   const int64_t rows = a.ix.tokens * a.hkv * a.group;
-  if (a.splits > 1) {
+  if (a.parts > 1) {
     a.ws_o = static_cast<float*>(ws);
-    a.ws_ml = a.ws_o + a.splits * rows * pd;
+    a.ws_ml = a.ws_o + a.parts * rows * pd;
   }
-  const int per = plan.tiles ? 32 * plan.waves : 16;
-  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1), (unsigned)a.hkv, (unsigned)a.splits);
+  const int per = plan.tiles ? 128 : 16;
+  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1), (unsigned)a.hkv, (unsigned)a.parts);
   if (plan.tiles) {
     if constexpr (sizeof(T) == 2) {
       switch (pd) {
@@ -663,7 +715,7 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
 #undef ROWS_CASE
   }
   NEURST_CHECK_LAUNCH("paged_attention");
-  if (a.splits > 1) {
+  if (a.parts > 1) {
     paged_attn_join<T><<<(unsigned)cdiv64(rows, 4), 256, 0, s>>>(a, pd, rows);
     NEURST_CHECK_LAUNCH("paged_attention join");
   }
@@ -692,7 +744,8 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   a.ws_o = a.ws_ml = nullptr;
   a.ldq = ldq; a.ldo = ldo; a.hkv = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.dh = (int)dh; a.causal = causal ? 1 : 0;
   const AttnPlan plan = attn_plan(tokens, batch, wide, page_size, kv_heads, a.group, dh, dtype, scale != 0.f);
-  a.splits = plan.splits;
+  a.parts = plan.parts;
+  a.part_keys = plan.part_keys;
   a.scale_log2 = scale * 1.44269504088896340736f;
   const int64_t need = neurst_paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype);
   NEURST_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
