@@ -11,13 +11,14 @@
 // 1e-11 of where real numbers put it (fp32 sums would move it by 1e-6, past a word in one draw of thirty).  Words below
 // 2^-45 of the best have weight 0 and are never drawn.
 //
-// The kept set is {key > K} and the first m words (by index) with key == K, keys being the logits in an order-preserving
-// integer form.  K is found by counting, not by sorting: a histogram over 2048 equal steps of (max - l) / T in [0, 32) - all
-// that can have weight - finds the step where the count passes top_k or the sum passes top_p, then the words of that one step
-// are counted again over the range of their keys until one key is left.
+// The kept set is {key > K} and the words with key == K up to a place, keys being the logits in an order-preserving integer
+// form.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in [0, 32) - all that can
+// have weight - finds the step where the count passes top_k or the sum passes top_p, and the words of that one step, a dozen
+// as a rule, are ranked among each other.  What top_k leaves (up to 1024 words) goes to a list in index order, and the rest of
+// the work runs on that.
 //
-// One workgroup a row; a row of up to 128 KB is read once, into shared memory, and every later pass runs on that.  Bound by
-// the chain of passes and barriers for few rows, by the fp64 exponentials (~25 instructions a word) for many.
+// One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
+// the chain of passes and barriers for few rows, by the fp64 exponentials (~25 instructions a word) for many without top_k.
 #include "common.h"
 
 struct SampleArgs {
@@ -36,7 +37,7 @@ struct SampleArgs {
 };
 
 typedef unsigned long long u64;
-constexpr int SAMPLE_BINS = 2048;
+constexpr int SAMPLE_BINS = 1024;
 constexpr double SAMPLE_ONE = 17592186044416.0;      // 2^44
 constexpr float SAMPLE_SPAN = 32.f;                   // e^-32 < 2^-45: rounds to 0
 
@@ -65,107 +66,327 @@ __device__ __forceinline__ u64 sample_weight(double x) {
   return __builtin_bit_cast(u64, v) & 0xFFFFFFFFFFFFFull;
 }
 
-__device__ __forceinline__ u64 shfl_u64(u64 v, int src) {
-  return (u64)(uint32_t)__shfl((int)(uint32_t)v, src, 64) | ((u64)(uint32_t)__shfl((int)(uint32_t)(v >> 32), src, 64) << 32);
+// ---- 64-lane scans through the DPP network (all lanes active) and sums over the waves of a workgroup ------------------------
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ u64 wave_scan_u64(u64 v, int lane) {      // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 x = shfl_u64(v, (lane - o) & 63);
-    if (lane >= o) v += x;
-  }
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 dpp_u64(u64 v) {
+  return (u64)dpp_u32<CTRL, ROWS>((uint32_t)v) | ((u64)dpp_u32<CTRL, ROWS>((uint32_t)(v >> 32)) << 32);
+}
+__device__ __forceinline__ u64 row_scan_u64(u64 v) {        // inclusive, within 16 lanes: shifts by 1, 2, 4, 8
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
   return v;
 }
-__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t x = (uint32_t)__shfl((int)v, (lane - o) & 63, 64);
-    if (lane >= o) v += x;
-  }
+__device__ __forceinline__ u64 wave_scan_u64(u64 v) {       // inclusive: then the rows' last lanes on to the rows behind them
+  v = row_scan_u64(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
   return v;
+}
+__device__ __forceinline__ u64 readlane_u64(u64 v, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) | ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32);
 }
 
-template <int NT> struct SampleShared {
+constexpr int SAMPLE_CAND = 256, SAMPLE_LIST = 1024;
+struct SampleCand { u64 w; uint32_t key; int at; };
+
+template <typename T, int NT> struct SampleShared {
   u64 hw[SAMPLE_BINS];
+  SampleCand cand[SAMPLE_CAND];
+  u64 ww[2][16], above, bin_w, drawn;
   uint32_t hc[SAMPLE_BINS];
-  u64 ww[16];
-  uint32_t wc[16], wa[16], wb[16];
+  int list_at[SAMPLE_LIST];
+  uint32_t wa[16], wb[16], bin_c, found_key, count;
   float wf[16];
-  int bin;
-  uint32_t above_c, bin_c;
-  u64 above_w, bin_w;
-  u64 seg[512];
-  int cut;
+  int bin, found_at, place;
+  T list[SAMPLE_LIST];
 };
 
-// The row, in shared memory (CACHED) or read again on every pass.  Wave w owns the words [w * span, (w + 1) * span), 64
-// neighbours at a time, so index order is wave, step, lane.
-template <typename T, int NT, bool CACHED> struct SampleRow {
-  const T* p;
-  int V, base, steps;
-  __device__ __forceinline__ float fetch(int i) const {
-    const int idx = base + i * 64;
-    const float x = CACHED || idx < V ? to_f32<T>(p[idx]) : -INFINITY;
-    return x == x ? x + 0.f : -INFINITY;           // NaN is never drawn; -0 counts as +0
-  }
-  __device__ __forceinline__ void init(const T* row, T* lds, int V_, int tid) {
-    V = V_;
-    steps = (V + NT - 1) / NT;
+// sum over the waves before this one and over all, from each wave's own sum (the same in all its lanes); one barrier; `slot`
+// alternates so that the next call need not wait for this one's readers
+template <typename S, int NW> __device__ __forceinline__ void waves_sum(S& s, int slot, u64 mine, int w, int lane, u64& before, u64& all) {
+  if (lane == 0) s.ww[slot][w] = mine;
+  __syncthreads();
+  const u64 inc = row_scan_u64(lane < NW ? s.ww[slot][lane] : 0);
+  all = readlane_u64(inc, NW - 1);
+  before = w ? readlane_u64(inc, w - 1) : 0;
+}
+
+// A sequence of words: place i of step and lane, in index order wave by wave, step by step, lane by lane.
+template <typename T, int NT> struct SampleView {
+  const T* p;                // [n]
+  int n, base, steps;
+  __device__ __forceinline__ void init(const T* p_, int n_, int tid) {
+    p = p_;
+    n = n_;
+    steps = (n + NT - 1) / NT;
     base = (tid >> 6) * steps * 64 + (tid & 63);
-    if constexpr (CACHED) {                        // every lane keeps to its own words: no barrier needed
-#pragma unroll 8
-      for (int i = 0; i < steps; ++i) {
-        const int idx = base + i * 64;
-        lds[idx] = idx < V ? row[idx] : (T)-INFINITY;
-      }
-      p = lds;
-    } else {
-      p = row;
-    }
+  }
+  __device__ __forceinline__ float at(int place) const {
+    const float x = place < n ? to_f32<T>(p[place]) : -INFINITY;
+    return x == x ? x + 0.f : -INFINITY;           // NaN is never drawn; -0 counts as +0
   }
   template <int UNROLL = 4, typename F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll UNROLL
-    for (int i = 0; i < steps; ++i) f(fetch(i), base + i * 64, i);
+    for (int i = 0; i < steps; ++i) f(at(base + i * 64), base + i * 64);
   }
 };
 
-// first bin at which the running count (or, by_weight, the running sum) reaches `need`, into s.bin / above_* / bin_*
-template <int NT> __device__ __forceinline__ void sample_cross(SampleShared<NT>& s, bool by_weight, u64 need, int tid) {
-  constexpr int PER = SAMPLE_BINS / NT;
+struct SampleRule {
+  float mx, bin_scale;
+  double inv_t;
+  u64 lowest;                // min_p as a weight
+  __device__ __forceinline__ u64 weight(float l) const {
+    if (l == mx) return (u64)SAMPLE_ONE;
+    const double x = ((double)l - (double)mx) * inv_t;
+    return x >= -SAMPLE_SPAN ? sample_weight(x) : 0;
+  }
+  // step of the histogram: grows as l falls, 0 for the best; SAMPLE_BINS: no weight
+  __device__ __forceinline__ int step_of(float l) const {
+    const float x = (mx - l) * bin_scale;
+    return l == mx ? 0 : (x < (float)SAMPLE_BINS ? (int)x : SAMPLE_BINS);
+  }
+};
+
+struct SampleLimit {         // words with key > K, and with key == K up to place `cut`
+  uint32_t K;
+  int cut;
+  __device__ __forceinline__ bool holds(uint32_t key, int place) const { return key > K || (key == K && place <= cut); }
+};
+
+// The word at which the running count (by_weight: the running sum), in descending order, reaches `need`: the new limit.
+// The histogram over the words that `lim` holds is in s.hc / s.hw.
+template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s, const SampleView<T, NT>& r,
+                                                                                                   const SampleRule& rule, SampleLimit lim, u64 need,
+                                                                                                   int tid) {
+  constexpr int NW = NT / 64, PER = SAMPLE_BINS / NT;
   const int lane = tid & 63, w = tid >> 6;
-  uint32_t c = 0;
-  u64 x = 0;
+  auto part = [&](int i) -> u64 { return BY_WEIGHT ? s.hw[i] : (u64)s.hc[i]; };
+  // the bin that reaches `need`, into s.bin, with the sum before it and its count
+  auto cross = [&](u64 want) {
+    u64 x = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) { c += s.hc[tid * PER + j]; x += s.hw[tid * PER + j]; }
-  const uint32_t ci = wave_scan_u32(c, lane);
-  const u64 xi = wave_scan_u64(x, lane);
-  if (lane == 63) { s.wc[w] = ci; s.ww[w] = xi; }
+    for (int j = 0; j < PER; ++j) x += part(tid * PER + j);
+    const u64 inc = wave_scan_u64(x);
+    u64 before, all;
+    waves_sum<SampleShared<T, NT>, NW>(s, 1, readlane_u64(inc, 63), w, lane, before, all);
+    u64 b = before + inc - x;
+    if (b < want && b + x >= want) {
+      for (int j = 0; j < PER; ++j) {
+        const u64 y = part(tid * PER + j);
+        if (b + y >= want) {
+          s.bin = tid * PER + j;
+          s.above = b;
+          s.bin_c = s.hc[tid * PER + j];
+          s.bin_w = y;
+          break;
+        }
+        b += y;
+      }
+    }
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+  };
+  cross(need);
+  const int bin = s.bin;
+  if (s.bin_c <= SAMPLE_CAND) {
+    // its words, ranked among each other
+    r.each([&](float l, int place) {
+      if (rule.step_of(l) == bin && l > -INFINITY) {
+        const uint32_t key = logit_key(l);
+        const u64 x = BY_WEIGHT ? rule.weight(l) : 1;
+        if (lim.holds(key, place) && x) {
+          const uint32_t at = atomicAdd(&s.count, 1u);       // the order does not matter
+          if (at < SAMPLE_CAND) s.cand[at] = SampleCand{x, key, place};
+        }
+      }
+    });
+    __syncthreads();
+    const int n = (int)s.bin_c;
+    if (tid < n) {
+      const SampleCand me = s.cand[tid];
+      u64 b = s.above;
+      for (int j = 0; j < n; ++j) {
+        const SampleCand c = s.cand[j];
+        if (c.key > me.key || (c.key == me.key && c.at < me.at)) b += c.w;
+      }
+      if (b < need && b + me.w >= need) {
+        s.found_key = me.key;
+        s.found_at = me.at;
+      }
+    }
+    __syncthreads();
+    return SampleLimit{s.found_key, s.found_at};
+  }
+  // very many words in one step (ties, or logits closer than 1 / 32 of the temperature): counted again over the range of
+  // their keys until one key is left, and that key's words by place
+  u64 above = s.above;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  r.each([&](float l, int place) {
+    if (rule.step_of(l) == bin && l > -INFINITY) {
+      const uint32_t k = logit_key(l);
+      if (lim.holds(k, place)) {
+        lo = k < lo ? k : lo;
+        hi = k > hi ? k : hi;
+      }
+    }
+  });
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t x = (uint32_t)__shfl_xor((int)lo, o, 64), y = (uint32_t)__shfl_xor((int)hi, o, 64);
+    lo = x < lo ? x : lo;
+    hi = y > hi ? y : hi;
+  }
+  if (lane == 0) { s.wa[w] = lo; s.wb[w] = hi; }
   __syncthreads();
-  uint32_t cb = ci - c;
-  u64 xb = xi - x;
-  for (int i = 0; i < w; ++i) { cb += s.wc[i]; xb += s.ww[i]; }
-  if (by_weight ? (xb < need && xb + x >= need) : ((u64)cb < need && (u64)cb + c >= need)) {
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t bc = s.hc[tid * PER + j];
-      const u64 bw = s.hw[tid * PER + j];
-      if (by_weight ? xb + bw >= need : (u64)cb + bc >= need) {
-        s.bin = tid * PER + j;
-        s.above_c = cb; s.above_w = xb;
-        s.bin_c = bc; s.bin_w = bw;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    lo = s.wa[i] < lo ? s.wa[i] : lo;
+    hi = s.wb[i] > hi ? s.wb[i] : hi;
+  }
+  while (lo < hi) {
+    const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;      // 1024 bins
+    __syncthreads();
+    for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
+    __syncthreads();
+    r.each([&](float l, int place) {
+      const uint32_t k = logit_key(l);
+      if (k >= lo && k <= hi && lim.holds(k, place)) {
+        const u64 x = rule.weight(l);
+        if (x || !BY_WEIGHT) {
+          atomicAdd(&s.hc[(hi - k) >> shift], 1u);
+          if (BY_WEIGHT) atomicAdd(&s.hw[(hi - k) >> shift], x);
+        }
+      }
+    });
+    __syncthreads();
+    cross(need - above);
+    above += s.above;
+    hi -= (uint32_t)s.bin << shift;
+    const uint32_t span = (1u << shift) - 1u;
+    if (hi - lo > span) lo = hi - span;
+  }
+  const uint32_t K = hi, ties = s.bin_c;
+  const u64 one = BY_WEIGHT ? s.bin_w / ties : 1;
+  const uint32_t m = (uint32_t)((need - above + one - 1) / one);      // of `ties` equal words the first m
+  uint32_t c = 0;
+  r.each([&](float l, int place) { c += logit_key(l) == K && place <= (lim.K == K ? lim.cut : 0x7fffffff) ? 1u : 0u; });
+  u64 before, all;
+  waves_sum<SampleShared<T, NT>, NW>(s, 0, readlane_u64(wave_scan_u64(c), 63), w, lane, before, all);
+  uint32_t seen = (uint32_t)before;
+  if (seen < m)
+    r.template each<1>([&](float l, int place) {
+      const u64 eq = __ballot(logit_key(l) == K);
+      const uint32_t here = (uint32_t)__popcll(eq);
+      if (seen < m && seen + here >= m && ((eq >> lane) & 1) && seen + (uint32_t)__popcll(eq & ((2ull << lane) - 1)) == m) s.found_at = place;
+      seen += here;
+    });
+  __syncthreads();
+  return SampleLimit{K, s.found_at};
+}
+
+// top-p and min-p over the words that `lim` holds, and the draw: the place drawn in s.place, its weight in s.drawn; returns
+// the sum of the words kept
+template <typename T, int NT> __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const SampleView<T, NT>& r, const SampleRule& rule,
+                                                                         SampleLimit lim, float top_p, float u, bool fresh, int tid) {
+  constexpr int NW = NT / 64;
+  typedef SampleShared<T, NT> S;
+  const int lane = tid & 63, w = tid >> 6;
+  u64 before, total;
+  if (top_p < 1.f) {
+    if (!fresh) {
+      __syncthreads();
+      for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
+      __syncthreads();
+    }
+    u64 mine = 0;
+    r.each([&](float l, int place) {
+      const u64 x = lim.holds(logit_key(l), place) ? rule.weight(l) : 0;
+      if (x) {
+        const int b = rule.step_of(l);                       // x != 0: below SAMPLE_BINS
+        atomicAdd(&s.hc[b], 1u);
+        atomicAdd(&s.hw[b], x);
+        mine += x;
+      }
+    });
+    waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
+    u64 need = (u64)ceil((double)top_p * (double)total);
+    if (need < 1) need = 1;
+    if (need < total) lim = sample_select<true>(s, r, rule, lim, need, tid);
+  }
+  auto kept = [&](float l, int place) -> u64 {
+    const u64 x = lim.holds(logit_key(l), place) ? rule.weight(l) : 0;
+    return x >= rule.lowest ? x : 0;
+  };
+  u64 mine = 0;
+  r.each([&](float l, int place) { mine += kept(l, place); });
+  const u64 own = readlane_u64(wave_scan_u64(mine), 63);
+  __syncthreads();                                           // the histogram and slot 0 are free
+  waves_sum<S, NW>(s, 0, own, w, lane, before, total);
+  u64 thr = (u64)((double)u * (double)total);
+  if (thr >= total) thr = total - 1;
+  if (before <= thr && thr < before + own && lane == 0) {    // this wave's words hold the draw
+    s.bin = w;
+    s.above = before;
+  }
+  __syncthreads();
+  // its steps' sums, dealt to all waves
+  const int first = s.bin * r.steps * 64 + lane;
+  for (int i = w; i < r.steps; i += NW) {
+    const u64 x = wave_scan_u64(kept(r.at(first + i * 64), first + i * 64));
+    if (lane == 63) s.hw[i] = x;
+  }
+  __syncthreads();
+  if (w == 0) {
+    u64 run = s.above;
+    int at = 0;
+    for (int j = 0; j < r.steps; j += 64) {                  // 64 steps at a time
+      const u64 x = j + lane < r.steps ? s.hw[j + lane] : 0, inc = run + wave_scan_u64(x);
+      const u64 over = __ballot(inc > thr);
+      if (over) {
+        at = j + __builtin_ctzll(over);
+        run = readlane_u64(inc - x, at - j);
         break;
       }
-      cb += bc;
-      xb += bw;
+      run = readlane_u64(inc, 63);
+    }
+    const int place = first + at * 64;
+    const u64 x = kept(r.at(place), place), c = run + wave_scan_u64(x);
+    if (c > thr && c - x <= thr) {
+      s.place = place;
+      s.drawn = x;
     }
   }
   __syncthreads();
+  return total;
 }
 
 template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT) sample_kernel(SampleArgs a) {
   constexpr int NW = NT / 64;
-  __shared__ SampleShared<NT> s;
+  typedef SampleShared<T, NT> S;
+  __shared__ S s;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t row = blockIdx.x;
+  extern __shared__ __attribute__((aligned(16))) char row_lds[];
+  const T* src = static_cast<const T*>(a.logits) + row * a.ld;
+  SampleView<T, NT> r;
+  r.init(CACHED ? reinterpret_cast<const T*>(row_lds) : src, a.V, tid);
+  float mx = -INFINITY;
+  if constexpr (CACHED) {                                   // every lane keeps to its own words: no barrier needed
+    T* dst = reinterpret_cast<T*>(row_lds);
+#pragma unroll 8
+    for (int i = 0; i < r.steps; ++i) {
+      const int at = r.base + i * 64;
+      const T x = at < a.V ? src[at] : (T)-INFINITY;
+      dst[at] = x;                                          // the image is padded to whole steps
+      const float l = to_f32<T>(x);
+      mx = l > mx ? l : mx;                                 // not for NaN
+    }
+  } else {
+    r.each([&](float l, int) { mx = fmaxf(mx, l); });
+  }
   float temp = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
   float top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
   float min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
@@ -177,226 +398,77 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   if (top_k <= 0 || top_k > a.V) top_k = a.V;
   float u = a.u[row];
   u = u > 0.f ? (u < 1.f ? u : 1.f) : 0.f;
-
-  extern __shared__ __attribute__((aligned(16))) char row_lds[];
-  SampleRow<T, NT, CACHED> r;
-  r.init(static_cast<const T*>(a.logits) + row * a.ld, reinterpret_cast<T*>(row_lds), a.V, tid);
   for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-  float mx = -INFINITY;
-  r.each([&](float l, int, int) { mx = fmaxf(mx, l); });
-  mx = wave_max(mx);
+  mx = wave_max(mx) + 0.f;
   if (lane == 0) s.wf[w] = mx;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < NW; ++i) mx = fmaxf(mx, s.wf[i]);
+  mx = wave_max(lane < NW ? s.wf[lane] : -INFINITY);
 
   int id = -1;
   float logp = -INFINITY;
-  if (mx > -INFINITY) {
-    const double inv_t = 1.0 / (double)temp;
-    const float bin_scale = (float)(SAMPLE_BINS / SAMPLE_SPAN * inv_t);
-    auto weight = [&](float l) -> u64 {
-      if (l == mx) return (u64)SAMPLE_ONE;
-      const double x = ((double)l - (double)mx) * inv_t;
-      return x >= -SAMPLE_SPAN ? sample_weight(x) : 0;
-    };
-    // step of the histogram: monotone in l, 0 for the best; words of the last step and below share it
-    auto step_of = [&](float l) -> int {
-      const float x = (mx - l) * bin_scale;
-      return l == mx ? 0 : (x < (float)(SAMPLE_BINS - 1) ? (int)x : SAMPLE_BINS - 1);
-    };
-    uint32_t K = 0;            // kept: key > K, or key == K and index <= cut
-    int cut = 0x7fffffff;
+  if (mx > -INFINITY && top_k == 1) {                       // the first maximum
+    int best = 0x7fffffff;
+    r.each([&](float l, int place) { best = l == mx && place < best ? place : best; });
+    for (int o = 32; o > 0; o >>= 1) {
+      const int x = __shfl_xor(best, o, 64);
+      best = x < best ? x : best;
+    }
+    if (lane == 0) s.wa[w] = (uint32_t)best;
+    __syncthreads();
+    id = (int)s.wa[0];
+    for (int i = 1; i < NW; ++i) id = (int)s.wa[i] < id ? (int)s.wa[i] : id;
+    logp = 0.f;
+  } else if (mx > -INFINITY) {
+    SampleRule rule;
+    rule.mx = mx;
+    rule.inv_t = 1.0 / (double)temp;
+    rule.bin_scale = (float)(SAMPLE_BINS / SAMPLE_SPAN * rule.inv_t);
+    rule.lowest = (u64)ceil((double)min_p * SAMPLE_ONE);
+    SampleLimit lim = {0u, 0x7fffffff};
     bool limited = false;
-    u64 kept_in_k = 0;         // the sum over the words top_k keeps
-    const bool by_k = top_k < a.V, by_p = top_p < 1.f;
-    uint32_t m = 0, ties = 0;  // of the words with key == K the first m are kept, there are `ties`
-    if (top_k == 1) {
-      uint32_t c = 0;
-      r.each([&](float l, int, int) { c += l == mx ? 1u : 0u; });
-      c = wave_scan_u32(c, lane);
-      if (lane == 63) s.wa[w] = c;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NW; ++i) ties += s.wa[i];
-      K = logit_key(mx);
-      m = 1;
-      limited = true;
-    } else {
-      // phase 0: the count reaches top_k; phase 1: the sum reaches top_p of what phase 0 kept
-      for (int phase = by_k ? 0 : 1; phase < (by_p ? 2 : 1); ++phase) {
-        u64 mine = 0;
-        uint32_t count = 0;
-        if (phase && by_k) {
-          __syncthreads();
-          for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-          __syncthreads();
+    if (top_k < a.V) {
+      uint32_t mine = 0;
+      r.each([&](float l, int) {
+        const int b = rule.step_of(l);
+        if (b < SAMPLE_BINS) {
+          atomicAdd(&s.hc[b], 1u);
+          ++mine;
         }
-        r.each([&](float l, int, int) {
-          const u64 x = logit_key(l) >= K ? weight(l) : 0;
-          if (x) {
-            const int b = step_of(l);
-            atomicAdd(&s.hc[b], 1u);
-            atomicAdd(&s.hw[b], x);
-            mine += x;
-            ++count;
-          }
-        });
-        mine = wave_scan_u64(mine, lane);
-        count = wave_scan_u32(count, lane);
-        if (lane == 63) { s.ww[w] = mine; s.wa[w] = count; }
-        __syncthreads();
-        u64 need = 0, n = 0;
-        if (phase == 0 || !by_k) kept_in_k = 0;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          if (phase == 0 || !by_k) kept_in_k += s.ww[i];
-          n += s.wa[i];
-        }
-        __syncthreads();
-        if (phase == 0) {
-          if (n <= (u64)top_k) continue;       // every word with weight stays
-          need = (u64)top_k;
-        } else {
-          need = (u64)ceil((double)top_p * (double)kept_in_k);
-          if (need < 1) need = 1;
-          if (need >= kept_in_k) continue;
-        }
-        // down to one key: ac / aw = words and sum before it, s.bin_c / s.bin_w = those that equal it
-        sample_cross<NT>(s, phase == 1, need, tid);
-        const int bin = s.bin;
-        uint32_t ac = s.above_c;
-        u64 aw = s.above_w;
-        uint32_t lo = 0xffffffffu, hi = 0;
-        r.each([&](float l, int, int) {
-          if (l > -INFINITY && step_of(l) == bin && weight(l)) {
-            const uint32_t k = logit_key(l);
-            lo = k < lo ? k : lo;
-            hi = k > hi ? k : hi;
-          }
-        });
-        for (int o = 32; o > 0; o >>= 1) {
-          const uint32_t x = (uint32_t)__shfl_xor((int)lo, o, 64), y = (uint32_t)__shfl_xor((int)hi, o, 64);
-          lo = x < lo ? x : lo;
-          hi = y > hi ? y : hi;
-        }
-        if (lane == 0) { s.wa[w] = lo; s.wb[w] = hi; }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-          lo = s.wa[i] < lo ? s.wa[i] : lo;
-          hi = s.wb[i] > hi ? s.wb[i] : hi;
-        }
-        while (lo < hi) {
-          const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 11 ? bits - 11 : 0;
-          for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-          __syncthreads();
-          r.each([&](float l, int, int) {
-            const uint32_t k = logit_key(l);
-            if (k >= lo && k <= hi) {
-              const u64 x = weight(l);
-              if (x) {
-                atomicAdd(&s.hc[(hi - k) >> shift], 1u);
-                atomicAdd(&s.hw[(hi - k) >> shift], x);
-              }
-            }
-          });
-          __syncthreads();
-          sample_cross<NT>(s, phase == 1, need - (phase == 1 ? aw : (u64)ac), tid);
-          ac += s.above_c;
-          aw += s.above_w;
-          hi -= (uint32_t)s.bin << shift;
-          const uint32_t span = (1u << shift) - 1u;
-          if (hi - lo > span) lo = hi - span;
-          __syncthreads();
-        }
-        K = hi;
-        ties = s.bin_c;
-        const u64 each = s.bin_w / ties;
-        if (phase == 0) {
-          m = (uint32_t)top_k - ac;
-          kept_in_k = aw + (u64)m * each;
-        } else {
-          m = (uint32_t)((need - aw + each - 1) / each);
-        }
-        limited = true;
-      }
-    }
-    __syncthreads();
-    if (limited && m < ties) {      // equal words: the first m by index
-      uint32_t c = 0;
-      r.each([&](float l, int, int) { c += logit_key(l) == K ? 1u : 0u; });
-      c = wave_scan_u32(c, lane);
-      if (lane == 63) s.wc[w] = c;
-      __syncthreads();
-      uint32_t before = 0;
-      for (int i = 0; i < w; ++i) before += s.wc[i];
-      if (before < m && before + s.wc[w] >= m) {
-        uint32_t seen = before;
-        r.template each<1>([&](float l, int idx, int) {
-          const u64 eq = __ballot(logit_key(l) == K);
-          const uint32_t here = (uint32_t)__popcll(eq);
-          if (seen < m && seen + here >= m) {
-            const bool mine_last = ((eq >> lane) & 1) && seen + (uint32_t)__popcll(eq & ((2ull << lane) - 1)) == m;
-            if (mine_last) s.cut = idx;
-          }
-          seen += here;
-        });
-      }
-      __syncthreads();
-      cut = s.cut;
-    }
-    const u64 lowest = (u64)ceil((double)min_p * SAMPLE_ONE);
-    auto kept = [&](float l, int idx) -> u64 {
-      const uint32_t k = logit_key(l);
-      if (limited && (k < K || (k == K && idx > cut))) return 0;
-      const u64 x = weight(l);
-      return x >= lowest ? x : 0;
-    };
-    u64 mine = 0;
-    r.each([&](float l, int idx, int) { mine += kept(l, idx); });
-    const u64 incl = wave_scan_u64(mine, lane);
-    if (lane == 63) s.ww[w] = incl;
-    for (int i = tid; i < 512; i += NT) s.seg[i] = 0;
-    __syncthreads();
-    u64 total = 0, before = 0;
-    for (int i = 0; i < NW; ++i) {
-      if (i < w) before += s.ww[i];
-      total += s.ww[i];
-    }
-    u64 thr = (u64)((double)u * (double)total);
-    if (thr >= total) thr = total - 1;
-    if (before <= thr && thr < before + s.ww[w]) {      // this wave holds the word: its step, then its lane
-      r.each([&](float l, int idx, int i) {
-        const u64 x = kept(l, idx);
-        if (x) atomicAdd(&s.seg[i], x);
       });
-      __threadfence_block();
-      u64 run = before;
-      int at = 0;
-      for (int j = 0; j < r.steps; j += 64) {           // 64 steps at a time
-        const u64 x = *(volatile u64*)&s.seg[j + lane], inc = run + wave_scan_u64(x, lane);
-        const u64 over = __ballot(inc > thr);
-        if (over) {
-          const int k = __builtin_ctzll(over);
-          at = j + k;
-          run = shfl_u64(inc - x, k);
-          break;
-        }
-        run = shfl_u64(inc, 63);
-      }
-      const int idx = r.base + at * 64;
-      const float l = r.fetch(at);
-      const u64 x = kept(l, idx);
-      const u64 c = run + wave_scan_u64(x, lane);
-      if (c > thr && c - x <= thr) {
-        s.cut = idx;
-        s.above_w = x;
-      }
+      u64 before, n;
+      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, n);
+      limited = n > (u64)top_k;                             // else every word with weight stays
+      if (limited) lim = sample_select<false>(s, r, rule, lim, (u64)top_k, tid);
     }
-    __syncthreads();
-    id = s.cut;
-    logp = (float)log((double)s.above_w / (double)total);
+    u64 total;
+    if (limited && top_k <= SAMPLE_LIST) {
+      uint32_t mine = 0;
+      r.each([&](float l, int place) { mine += lim.holds(logit_key(l), place) ? 1u : 0u; });
+      u64 before, n;
+      __syncthreads();
+      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, n);
+      int at = (int)before;
+      r.template each<1>([&](float l, int place) {
+        const u64 in = __ballot(lim.holds(logit_key(l), place));
+        if ((in >> lane) & 1) {
+          const int k = at + __popcll(in & ((1ull << lane) - 1));
+          if (k < SAMPLE_LIST) {
+            s.list[k] = (T)l;
+            s.list_at[k] = place;
+          }
+        }
+        at += __popcll(in);
+      });
+      __syncthreads();
+      SampleView<T, NT> few;
+      few.init(s.list, (int)n, tid);
+      total = sample_draw(s, few, rule, SampleLimit{0u, 0x7fffffff}, top_p, u, false, tid);
+      id = s.list_at[s.place];
+    } else {
+      total = sample_draw(s, r, rule, lim, top_p, u, top_k >= a.V, tid);
+      id = s.place;
+    }
+    logp = (float)log((double)s.drawn / (double)total);
   }
   if (tid == 0) {
     if (!a.preds) {
@@ -419,10 +491,11 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
 }
 
 template <typename T> static int sample_launch(const SampleArgs& a, int64_t rows, hipStream_t s) {
-  // 1024 threads once a row gives each of them four words; 128 KB of shared memory hold the row beside the histogram
+  // 1024 threads once a row gives each of them four words; 132 KB of shared memory hold the row beside the histogram
   const int nt = a.V > 4096 ? 1024 : 256;
   const int64_t padded = cdiv64(a.V, nt) * nt, bytes = padded * (int64_t)sizeof(T);
-  const bool cached = bytes <= 128 * 1024;
+  const bool cached = bytes <= 132 * 1024;
+  static_assert(sizeof(SampleShared<T, 1024>) + 132 * 1024 <= 160 * 1024, "shared memory of a CU");
 #define SAMPLE_CASE(N, C)                                                                                              \
   do {                                                                                                                 \
     if (C && bytes > 32 * 1024) {                                                                                      \
