@@ -17,8 +17,6 @@
 // memory by direct loads, one tile ahead of the one in use, and all waves read them from there.  The same transposed
 // products with the 32 x 32 x 16 instruction; the key that sits in row r of a 32-key block is chosen again so that a lane's
 // results are runs of eight consecutive keys.
-#include <type_traits>
-
 #include "paged.h"
 
 struct PagedAttnArgs {
@@ -30,6 +28,8 @@ struct PagedAttnArgs {
   int64_t ldq, ldo;
   int hkv, group, dh, causal;
   int parts, part_keys;     // the keys in parts of part_keys, one workgroup each
+  int32_t* order;           // tiles in the order of their work, most first (null: as they come)
+  int64_t tiles;            // of rows, an upper bound
   float scale_log2;         // scale * log2(e): exp(x) = exp2(x log2(e))
 };
 
@@ -96,9 +96,10 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 128 ? 2 : 1) pag
   __shared__ float red[NW][16][LD];
   __shared__ float ml[NW][16][2];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y, z = blockIdx.z;
+  // heads first: with a multiple of eight of them, or a divisor, an XCD sees few heads' keys through its L2
+  const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
   RowTile t;
-  if (!row_tile<16>(a, blockIdx.x, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  if (!row_tile<16>(a, blockIdx.x / (unsigned)a.hkv, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
   const int dh = EXACT ? DH : a.dh;
   const int page = 1 << a.ix.page_log2, pmask = page - 1;
   // this lane's query: row m of the tile
@@ -325,6 +326,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 128 ? 2 : 1) pag
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+constexpr int SG_VALU = 2, SG_MFMA = 8, SG_READ = 0x100;      // classes of __builtin_amdgcn_sched_group_barrier
 
 // An image of rows of NC 16-byte chunks: chunk c of row r lies at another place of the row, chosen by r / PER - PER being the
 // rows after which the 256 bytes of all banks come round again - so that the lanes of a read, neighbouring rows with one
@@ -332,6 +334,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 template <int NC> struct Image {
   static constexpr int PER = NC % 16 == 0 ? 1 : NC % 8 == 0 ? 2 : 4;
   static constexpr bool XOR = (NC & (NC - 1)) == 0;
+  // (of 32 rows more the same where XOR)
   static __device__ __forceinline__ int place(int r, int c) {
     if constexpr (XOR) return c ^ ((r / PER) & (NC - 1));
     const int x = c + (r / PER) % NC;
@@ -357,9 +360,11 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
   typedef Image<8> VI;
   extern __shared__ __attribute__((aligned(1024))) char smem[];                 // [2][keys, values]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
-  const int kvh = blockIdx.y, z = blockIdx.z;
+  const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
   RowTile t;
-  if (!row_tile<ROWS>(a, blockIdx.x, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  int64_t tile = blockIdx.x / (unsigned)a.hkv;
+  if (a.order) tile = a.order[tile];
+  if (!row_tile<ROWS>(a, tile, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
   const int dh = EXACT ? DH : a.dh;
   const int page = 1 << a.ix.page_log2, pmask = page - 1;
   const int row = 32 * w + m;
@@ -387,6 +392,8 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
       w_end = t.shift + (t.row_begin + 32 * w + (w_rows < 32 ? w_rows : 32) - 1) / a.group + 1;
       w_min = t.shift + (t.row_begin + 32 * w) / a.group + 1;
     }
+    w_end = __builtin_amdgcn_readfirstlane(w_end);
+    w_min = __builtin_amdgcn_readfirstlane(w_min);
   }
   const int nt = (t.kv_end + KT - 1) / KT, per = a.part_keys / KT;
   const int t0 = z * per, t1 = t0 + per < nt ? t0 + per : nt;
@@ -453,29 +460,35 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float mx = -INFINITY, l = 0.f;      // maximum in units of log2, sum of this lane's half
 
-  auto compute = [&](int ti, int buf, int ids, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
+  auto compute = [&](int ti, int buf, int ids, bool full) __attribute__((always_inline)) {
     const char* kimg = smem + buf * 2 * IMG;
     const char* vimg = kimg + IMG;
     const int base = ti * KT;
     int mm = m;
     asm volatile("" : "+v"(mm));                           // image addresses are made here, not kept over the loop
+    mm &= 31;
+    auto keys = [&](int b, int st) {
+      bf16x8 k = *reinterpret_cast<const bf16x8*>(kimg + 32 * b * NC * 16 + (mm * NC + KI::place(KI::XOR ? mm : 32 * b + mm, 2 * st + h)) * 16);
+      if (!EXACT && 16 * st + 8 * h >= dh) k = bf16x8{};
+      return k;
+    };
     f32x16 s[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+      for (int st = 0; st < STEPS; ++st) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(b, st), qf[st], st ? s[b] : f32x16{}, 0, 0, 0);
+    // reads four ahead of the products
+    if constexpr (EXACT) {
+      __builtin_amdgcn_sched_group_barrier(SG_READ, 4, 0);
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) {
-        const int rr = 32 * b + mm;
-        bf16x8 k = *reinterpret_cast<const bf16x8*>(kimg + (rr * NC + KI::place(rr, 2 * st + h)) * 16);
-        if (!EXACT && 16 * st + 8 * h >= dh) k = bf16x8{};
-        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[st], s[b], 0, 0, 0);
+      for (int i = 0; i < 2 * STEPS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+        if (i + 4 < 2 * STEPS) __builtin_amdgcn_sched_group_barrier(SG_READ, 1, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
     unsigned okay = 0xf;
-    if constexpr (MASKED) {
+    if (!full) {
       okay = (unsigned)(__ballot(ids >= 0) & 0xf);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -499,32 +512,45 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
       mx = mn;
     }
     const float mu = safe_max(mx);
-    bf16x8 p[4];
     float sum = 0.f;
+    auto weights = [&](int ks) {
+      bf16x8 p;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float pe = fast_exp2(fmaf(s[i >> 4][i & 15], c_abs, -mu));
-      sum += pe;
-      p[i >> 3][i & 7] = (bf16_t)pe;       // rounded for the second product only, as in the other kernel
-    }
-    l += sum;
-    __builtin_amdgcn_sched_barrier(0);
-    auto values = [&](int ks, int d) {
-      const int rr = 32 * d + mm;
-      return *reinterpret_cast<const bf16x8*>(vimg + (rr * 8 + VI::place(rr, 2 * ks + h)) * 16);
+      for (int e = 0; e < 8; ++e) {
+        const float pe = fast_exp2(fmaf(s[ks >> 1][8 * (ks & 1) + e], c_abs, -mu));
+        sum += pe;
+        p[e] = (bf16_t)pe;                 // rounded for the second product only, as in the other kernel
+      }
+      return p;
     };
-    if constexpr (!MASKED) {
+    auto values = [&](int ks, int d) {
+      return *reinterpret_cast<const bf16x8*>(vimg + 32 * d * 128 + (mm * 8 + VI::place(mm, 2 * ks + h)) * 16);
+    };
+    if (full) {
+      // sixteen keys at a time: their products run while the vector unit makes the weights of the next sixteen
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
+        const bf16x8 p = weights(ks);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(ks, d), p[ks], acc[d], 0, 0, 0);
-        if (ks & 1) __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(ks, d), p, acc[d], 0, 0, 0);
       }
+      if constexpr (DH <= 192) {
+        __builtin_amdgcn_sched_group_barrier(SG_READ, ND < 4 ? ND : 4, 0);
+        __builtin_amdgcn_sched_group_barrier(SG_VALU, 28, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * ND; ++i) {
+          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(SG_READ, 1, 0);
+          if (i < 3 * ND) __builtin_amdgcn_sched_group_barrier(SG_VALU, (28 + ND - 1) / ND, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     } else {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const int k0 = base + 16 * ks + 8 * h;
         const bool ok = okay >> ks & 1;
+        const bf16x8 p = weights(ks);
         bf16x8 seen;
 #pragma unroll
         for (int e = 0; e < 8; ++e) seen[e] = (bf16_t)(ok && k0 + e < vis ? 1.f : 0.f);
@@ -555,11 +581,12 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
               if (nd[i] > 0.f) acc[d][i] -= INFINITY;
             }
           }
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[ks], acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, acc[d], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+    l += sum;
   };
 
   int ids = pages_of(t0);
@@ -571,8 +598,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
     if (ti + 1 < t1) issue(ti + 1, buf ^ 1, next);
     const int base = ti * KT;
     if (base < w_end) {
-      if (base + KT <= w_min && (__ballot(ids >= 0) & 0xf) == 0xf) compute(ti, buf, ids, std::false_type());
-      else compute(ti, buf, ids, std::true_type());
+      compute(ti, buf, ids, base + KT <= w_min && (__ballot(ids >= 0) & 0xf) == 0xf);
     }
     ids = next;
   }
@@ -606,6 +632,49 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
       a.ws_ml[2 * wrow + 1] = l;
     }
   }
+}
+
+// Tiles by the keys their rows see, most first, so that the last workgroups to start are short ones: a causal batch of three
+// sequences of 3600 to 9000 tokens leaves a quarter of the chip's time idle in the order it comes, a twentieth like this.
+// One workgroup, a counting sort over 1024 classes; which of two tiles of a class comes first does not matter.
+__global__ void __launch_bounds__(1024) paged_attn_order(PagedAttnArgs a, int rows) {
+  __shared__ uint32_t first[1024];
+  __shared__ uint32_t sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  first[tid] = 0;
+  __syncthreads();
+  const int64_t most = (((int64_t)a.ix.wide << a.ix.page_log2) + 1023) >> 10;      // keys of a class
+  auto class_of = [&](int64_t tile) {
+    int lo = 0, hi = a.ix.batch;                            // the last sequence that starts at or before the tile
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (paged_tile_start(a.ix.cu[mid], a.group, rows, 1, mid) <= tile) lo = mid;
+      else hi = mid;
+    }
+    const PagedSeq s = paged_seq(a.ix, lo);
+    const int64_t own = tile - paged_tile_start(a.ix.cu[lo], a.group, rows, 1, lo), total = (int64_t)s.new_tokens * a.group;
+    if (own < 0 || own * rows >= total) return 1023;        // nothing to do
+    const int64_t last = (own + 1) * rows < total ? ((own + 1) * rows - 1) / a.group : s.new_tokens - 1;
+    const int64_t keys = a.causal && s.ctx ? s.ctx - s.new_tokens + last + 1 : s.ctx;
+    const int64_t c = keys / most;
+    return 1023 - (int)(c < 1023 ? c : 1023);
+  };
+  for (int64_t i = tid; i < a.tiles; i += 1024) atomicAdd(&first[class_of(i)], 1u);
+  __syncthreads();
+  const uint32_t mine = first[tid];
+  uint32_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t x = (uint32_t)__shfl((int)inc, (lane - o) & 63, 64);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 63) sums[w] = inc;
+  __syncthreads();
+  uint32_t before = inc - mine;
+  for (int i = 0; i < w; ++i) before += sums[i];
+  first[tid] = before;
+  __syncthreads();
+  for (int64_t i = tid; i < a.tiles; i += 1024) a.order[atomicAdd(&first[class_of(i)], 1u)] = (int32_t)i;
 }
 
 // joins the parts: one wave a row (token x head)
@@ -647,7 +716,7 @@ static int padded_dh(int64_t dh) {
 
 // What a call launches, from its sizes alone (the lengths are on the device): the kernel by the rows an average sequence
 // brings to a key/value head, and into how many parts the keys are split so that the chip is filled.
-struct AttnPlan { int tiles, parts, part_keys; };
+struct AttnPlan { int tiles, parts, part_keys, order; };
 static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group, int64_t dh, int dtype,
                           bool scaled) {
   AttnPlan p;
@@ -660,16 +729,22 @@ static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t p
   if (part * 64 < keys) part = cdiv64(cdiv64(keys, 64), least) * least;
   p.part_keys = (int)(part < keys ? part : cdiv64(keys, 64) * 64);
   p.parts = (int)cdiv64(keys, p.part_keys);
+  // sorted by work where more workgroups are launched than run at once (two a CU)
+  p.order = p.tiles && p.parts == 1 && wgs > 512 && paged_tiles(tokens, batch, group, 128, 1) <= (1 << 16);
   return p;
+}
+static int64_t plan_bytes(const AttnPlan& p, int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t dh) {
+  if (p.order) return paged_tiles(tokens, batch, group, 128, 1) * 4;
+  return p.parts <= 1 ? 0 : (int64_t)p.parts * tokens * q_heads * (padded_dh(dh) + 2) * 4;
 }
 
 extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t q_heads,
                                                           int64_t kv_heads, int64_t dh, int dtype) {
   if (tokens <= 0 || batch <= 0 || wide <= 0 || page_size <= 0 || q_heads <= 0 || kv_heads <= 0 || dh <= 0 || dh > 256) return 0;
   const int64_t group = q_heads / kv_heads;
-  const int a = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, true).parts;
-  const int b = attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, false).parts, s = a > b ? a : b;
-  return s <= 1 ? 0 : (int64_t)s * tokens * q_heads * (padded_dh(dh) + 2) * 4;
+  const int64_t a = plan_bytes(attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, true), tokens, batch, q_heads, group, dh);
+  const int64_t b = plan_bytes(attn_plan(tokens, batch, wide, page_size, kv_heads, group, dh, dtype, false), tokens, batch, q_heads, group, dh);
+  return a > b ? a : b;
 }
 
 template <int DH> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
@@ -691,7 +766,13 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
     a.ws_ml = a.ws_o + a.parts * rows * pd;
   }
   const int per = plan.tiles ? 128 : 16;
-  const dim3 grid((unsigned)paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1), (unsigned)a.hkv, (unsigned)a.parts);
+  a.tiles = paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1);
+  const dim3 grid((unsigned)(a.tiles * a.hkv), (unsigned)a.parts);
+  if (plan.order) {
+    a.order = static_cast<int32_t*>(ws);
+    paged_attn_order<<<1, 1024, 0, s>>>(a, per);
+    NEURST_CHECK_LAUNCH("paged_attention order");
+  }
   if (plan.tiles) {
     if constexpr (sizeof(T) == 2) {
       switch (pd) {
@@ -731,7 +812,8 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   PAGED_CHECK_INDEX("paged_attention");
   NEURST_CHECK_ARG(kv_heads > 0 && kv_heads <= 4096 && q_heads > 0 && q_heads <= 65536 && q_heads % kv_heads == 0,
                    "paged_attention: q_heads must be a multiple of kv_heads");
-  NEURST_CHECK_ARG(tokens * (q_heads / kv_heads) <= INT32_MAX, "paged_attention: too many rows");
+  NEURST_CHECK_ARG((tokens * (q_heads / kv_heads) / 16 + batch) * kv_heads <= INT32_MAX && tokens * (q_heads / kv_heads) <= INT32_MAX,
+                   "paged_attention: too many rows");
   NEURST_CHECK_ARG(ldq >= q_heads * dh && ldo >= q_heads * dh, "paged_attention: a row stride is smaller than its heads");
   NEURST_CHECK_ARG(scale == scale && scale <= 3.4e38f && scale >= -3.4e38f, "paged_attention: scale must be finite");
   const int64_t es = (int64_t)dtype_size(dtype);
@@ -742,6 +824,7 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages);
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.o = o; a.status = status;
   a.ws_o = a.ws_ml = nullptr;
+  a.order = nullptr;
   a.ldq = ldq; a.ldo = ldo; a.hkv = (int)kv_heads; a.group = (int)(q_heads / kv_heads); a.dh = (int)dh; a.causal = causal ? 1 : 0;
   const AttnPlan plan = attn_plan(tokens, batch, wide, page_size, kv_heads, a.group, dh, dtype, scale != 0.f);
   a.parts = plan.parts;
