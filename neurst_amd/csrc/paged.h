@@ -3,12 +3,25 @@
 #include "common.h"
 #include "paged_index.h"
 
-// paged_search with one wave counting 64 candidates at a time
-__device__ __forceinline__ int paged_find(const PagedIndex& x, int64_t tile, int64_t mult, int64_t per, int64_t extra, int lane) {
-  return paged_search(x.batch, [&](int lo, int step, int width) {
-    const int b = lo + lane * step;
-    return (int)__popcll(__ballot(lane * step < width && paged_tile_start(x.cu[b], mult, per, extra, b) <= tile));
+// paged_search with one wave counting 64 candidates at a time, and the lengths of the sequence found: the lanes of the last
+// round load those of their candidates along with its start, so that one trip to memory serves both (batches up to 64)
+__device__ __forceinline__ int paged_locate(const PagedIndex& x, int64_t tile, int64_t mult, int64_t per, int64_t extra, int lane, PagedSeq& s) {
+  int first = 0;
+  int32_t begin = 0, end = 0, ctx = 0;
+  const int b = paged_search(x.batch, [&](int lo, int step, int width) {
+    const int c = lo + lane * step;
+    const bool in = lane * step < width;
+    first = lo;
+    if (in) {
+      begin = x.cu[c];
+      end = x.cu[c + 1];
+      ctx = x.ctx[c];
+    }
+    return (int)__popcll(__ballot(in && paged_tile_start(begin, mult, per, extra, c) <= tile));
   });
+  const int at = b < 0 ? 0 : (b - first) & 63;      // the last round steps by one
+  s = paged_seq_of(x, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), __builtin_amdgcn_readlane(ctx, at));
+  return b;
 }
 
 __device__ __forceinline__ void paged_report(int32_t* status, int bits) {

@@ -31,12 +31,12 @@ constexpr int APPEND_TILE = 64;
 template <typename T, int VEC> __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
   constexpr int E = 16 / sizeof(T);          // slots of a value item, and its columns
   const int lane = threadIdx.x & 63;
-  const int b = paged_find(a.ix, blockIdx.x, 1, APPEND_TILE, 2, lane);
+  PagedSeq s;
+  const int b = paged_locate(a.ix, blockIdx.x, 1, APPEND_TILE, 2, lane, s);
   if (b < 0) return;
-  const PagedSeq s = paged_seq(a.ix, b);
   if (s.bad && blockIdx.y == 0 && threadIdx.x == 0) paged_report(a.status, s.bad);
   if (s.ctx == 0 || s.new_tokens == 0) return;
-  const int64_t tile = blockIdx.x - paged_tile_start(a.ix.cu[b], 1, APPEND_TILE, 2, b);
+  const int64_t tile = blockIdx.x - paged_tile_start(s.cu, 1, APPEND_TILE, 2, b);
   const int first = s.ctx - s.new_tokens;                                  // position of the first new token
   const int64_t lo64 = (int64_t)(first & ~(APPEND_TILE - 1)) + tile * APPEND_TILE;
   if (lo64 >= s.ctx) return;

@@ -61,11 +61,11 @@ struct RowTile {
   int row_begin;                                              // first of the tile's rows within the sequence
 };
 template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs& a, int64_t tile, int lane, RowTile& t, bool report) {
-  t.b = paged_find(a.ix, tile, a.group, ROWS, 1, lane);
+  PagedSeq s;
+  t.b = paged_locate(a.ix, tile, a.group, ROWS, 1, lane, s);
   if (t.b < 0) return false;
-  const PagedSeq s = paged_seq(a.ix, t.b);
   if (report && s.bad) paged_report(a.status, s.bad);
-  const int64_t own = tile - paged_tile_start(a.ix.cu[t.b], a.group, ROWS, 1, t.b);
+  const int64_t own = tile - paged_tile_start(s.cu, a.group, ROWS, 1, t.b);
   const int64_t rows = (int64_t)s.new_tokens * a.group;
   if (own * ROWS >= rows) return false;
   t.row_begin = (int)(own * ROWS);
@@ -88,7 +88,7 @@ __device__ __forceinline__ void part_nothing(const PagedAttnArgs& a, const RowTi
 }
 
 template <typename T, int DH, bool EXACT, int NW>
-__global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 128 ? 2 : 1) paged_attn_rows(PagedAttnArgs a) {
+__global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 128 ? 2 : 1) paged_attn_rows(PagedAttnArgs a) {
   typedef PagedMma<T> A;
   typedef typename A::V V;
   constexpr int E = A::E, KT = A::KT, NSUB = A::NSUB, KC = DH / (4 * E), ND = DH / 16;
@@ -716,25 +716,29 @@ static int padded_dh(int64_t dh) {
 
 // What a call launches, from its sizes alone (the lengths are on the device): the kernel by the rows an average sequence
 // brings to a key/value head, and into how many parts the keys are split so that the chip is filled.
-struct AttnPlan { int tiles, parts, part_keys, order; };
+struct AttnPlan { int tiles, waves, parts, part_keys, order; };
+static int plan_rows(const AttnPlan& p) { return p.tiles ? 32 * p.waves : 16; }
 static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group, int64_t dh, int dtype,
                           bool scaled) {
   AttnPlan p;
   const int64_t rows = cdiv64(tokens, batch) * group, keys = wide * page_size;
   p.tiles = dtype == NEURST_BF16 && scaled && rows > 32;
-  const int64_t wgs = batch * cdiv64(rows, p.tiles ? 128 : 16) * kv_heads;
-  // parts of equal length, not of equal number a sequence: the workgroups of a ragged batch then take equally long
+  p.waves = rows > 64 ? 4 : 2;                                  // of 32 rows
+  const int64_t wgs = batch * cdiv64(rows, plan_rows(p)) * kv_heads;
+  // parts of equal length, not of equal number a sequence: the workgroups of a ragged batch then take equally long.  A second
+  // launch joins them (4 us), so up to 1024 keys stay whole.
   const int64_t least = p.tiles ? 1024 : 512, want = p.tiles ? 512 : 4096;
   int64_t part = cdiv64(cdiv64(keys * wgs, want), least) * least;
-  if (part * 64 < keys) part = cdiv64(cdiv64(keys, 64), least) * least;
-  p.part_keys = (int)(part < keys ? part : cdiv64(keys, 64) * 64);
+  if (part * 64 < keys) part = cdiv64(keys, 64);
+  if (part >= keys || keys <= 1024) part = keys;
+  p.part_keys = (int)(cdiv64(cdiv64(keys, cdiv64(keys, part)), 64) * 64);
   p.parts = (int)cdiv64(keys, p.part_keys);
   // sorted by work where more workgroups are launched than run at once (two a CU)
-  p.order = p.tiles && p.parts == 1 && wgs > 512 && paged_tiles(tokens, batch, group, 128, 1) <= (1 << 16);
+  p.order = p.tiles && p.parts == 1 && wgs > 512 && paged_tiles(tokens, batch, group, plan_rows(p), 1) <= (1 << 16);
   return p;
 }
 static int64_t plan_bytes(const AttnPlan& p, int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t dh) {
-  if (p.order) return paged_tiles(tokens, batch, group, 128, 1) * 4;
+  if (p.order) return paged_tiles(tokens, batch, group, plan_rows(p), 1) * 4;
   return p.parts <= 1 ? 0 : (int64_t)p.parts * tokens * q_heads * (padded_dh(dh) + 2) * 4;
 }
 
@@ -747,8 +751,8 @@ extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_
   return a > b ? a : b;
 }
 
-template <int DH> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
-  constexpr int NW = 4, LDS = 2 * 2 * 64 * DH * 2;
+template <int DH, int NW> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
+  constexpr int LDS = 2 * 2 * 64 * DH * 2;
   auto kernel = a.dh == DH ? paged_attn_tiles<DH, true, NW> : paged_attn_tiles<DH, false, NW>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -765,7 +769,7 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
     a.ws_o = static_cast<float*>(ws);
     a.ws_ml = a.ws_o + a.parts * rows * pd;
   }
-  const int per = plan.tiles ? 128 : 16;
+  const int per = plan_rows(plan);
   a.tiles = paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1);
   const dim3 grid((unsigned)(a.tiles * a.hkv), (unsigned)a.parts);
   if (plan.order) {
@@ -776,12 +780,12 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   if (plan.tiles) {
     if constexpr (sizeof(T) == 2) {
       switch (pd) {
-        case 32: if (int e = tiles_launch<32>(a, grid, s)) return e; break;
-        case 64: if (int e = tiles_launch<64>(a, grid, s)) return e; break;
-        case 96: if (int e = tiles_launch<96>(a, grid, s)) return e; break;
-        case 128: if (int e = tiles_launch<128>(a, grid, s)) return e; break;
-        case 192: if (int e = tiles_launch<192>(a, grid, s)) return e; break;
-        case 256: if (int e = tiles_launch<256>(a, grid, s)) return e; break;
+        case 32: if (int e = plan.waves == 2 ? tiles_launch<32, 2>(a, grid, s) : tiles_launch<32, 4>(a, grid, s)) return e; break;
+        case 64: if (int e = plan.waves == 2 ? tiles_launch<64, 2>(a, grid, s) : tiles_launch<64, 4>(a, grid, s)) return e; break;
+        case 96: if (int e = plan.waves == 2 ? tiles_launch<96, 2>(a, grid, s) : tiles_launch<96, 4>(a, grid, s)) return e; break;
+        case 128: if (int e = plan.waves == 2 ? tiles_launch<128, 2>(a, grid, s) : tiles_launch<128, 4>(a, grid, s)) return e; break;
+        case 192: if (int e = plan.waves == 2 ? tiles_launch<192, 2>(a, grid, s) : tiles_launch<192, 4>(a, grid, s)) return e; break;
+        case 256: if (int e = plan.waves == 2 ? tiles_launch<256, 2>(a, grid, s) : tiles_launch<256, 4>(a, grid, s)) return e; break;
       }
     }
   } else {

@@ -31,30 +31,31 @@ struct PagedSeq {
   int new_tokens; // rows of this sequence (0: nothing to do)
   int ctx;        // tokens in the cache with them (0: nothing visible)
   int bad;
+  int32_t cu;     // cu[b] as it is
 };
 
 // Lengths of sequence b.  Rows out of range: the sequence is left out.  A cache shorter than the rows it should hold, or
 // longer than the page table: the rows exist but nothing is visible to them.
-NEURST_HD PagedSeq paged_seq(const PagedIndex& x, int b) {
+NEURST_HD PagedSeq paged_seq_of(const PagedIndex& x, int32_t begin, int32_t end, int32_t ctx) {
   PagedSeq s;
-  const int64_t a = x.cu[b], e = x.cu[b + 1];
-  s.row0 = a;
+  s.row0 = begin;
   s.bad = 0;
   s.new_tokens = 0;
   s.ctx = 0;
-  if (a < 0 || e < a || e > x.tokens) {
+  s.cu = begin;
+  if (begin < 0 || end < begin || end > x.tokens) {
     s.bad = PAGED_BAD_LENGTH;
     return s;
   }
-  s.new_tokens = (int)(e - a);
-  const int64_t c = x.ctx[b];
-  if (c < s.new_tokens || c > ((int64_t)x.wide << x.page_log2)) {
+  s.new_tokens = end - begin;
+  if (ctx < s.new_tokens || ctx > ((int64_t)x.wide << x.page_log2)) {
     s.bad = PAGED_BAD_LENGTH;
     return s;
   }
-  s.ctx = (int)c;
+  s.ctx = ctx;
   return s;
 }
+NEURST_HD PagedSeq paged_seq(const PagedIndex& x, int b) { return paged_seq_of(x, x.cu[b], x.cu[b + 1], x.ctx[b]); }
 
 // page of position p (0 <= p < wide << page_log2 is the caller's to hold), -1 for an id outside the pool
 NEURST_HD int paged_page(const PagedIndex& x, int b, int p) {
