@@ -733,6 +733,8 @@ static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t p
   if (part >= keys || keys <= 1024) part = keys;
   p.part_keys = (int)(cdiv64(cdiv64(keys, cdiv64(keys, part)), 64) * 64);
   p.parts = (int)cdiv64(keys, p.part_keys);
+  // few workgroups: eight waves in each
+  if (!p.tiles) p.waves = wgs * p.parts <= 256 ? 8 : 4;
   // sorted by work where more workgroups are launched than run at once (two a CU)
   p.order = p.tiles && p.parts == 1 && wgs > 512 && paged_tiles(tokens, batch, group, plan_rows(p), 1) <= (1 << 16);
   return p;
@@ -791,8 +793,13 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   } else {
 #define ROWS_CASE(D)                                                                       \
   case D:                                                                                  \
-    if (a.dh == D) paged_attn_rows<T, D, true, 4><<<grid, 256, 0, s>>>(a);                  \
-    else paged_attn_rows<T, D, false, 4><<<grid, 256, 0, s>>>(a);                           \
+    if (plan.waves == 8) {                                                                 \
+      if (a.dh == D) paged_attn_rows<T, D, true, 8><<<grid, 512, 0, s>>>(a);                \
+      else paged_attn_rows<T, D, false, 8><<<grid, 512, 0, s>>>(a);                         \
+    } else {                                                                               \
+      if (a.dh == D) paged_attn_rows<T, D, true, 4><<<grid, 256, 0, s>>>(a);                \
+      else paged_attn_rows<T, D, false, 4><<<grid, 256, 0, s>>>(a);                         \
+    }                                                                                      \
     break;
     switch (pd) {
       ROWS_CASE(32) ROWS_CASE(64) ROWS_CASE(96) ROWS_CASE(128) ROWS_CASE(192) ROWS_CASE(256)
