@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-constexpr int SG_VALU = 2, SG_MFMA = 8, SG_READ = 0x100;      // classes of __builtin_amdgcn_sched_group_barrier
+constexpr int AHEAD = 4;      // fragments read from shared memory ahead of their product
 
 // An image of rows of NC 16-byte chunks: chunk c of row r lies at another place of the row, chosen by r / PER - PER being the
 // rows after which the 256 bytes of all banks come round again - so that the lanes of a read, neighbouring rows with one
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
   constexpr int ROWS = 32 * NW, KT = 64, NC = DH / 8, STEPS = DH / 16, ND = DH / 32, IMG = KT * DH * 2;
   typedef Image<NC> KI;
   typedef Image<8> VI;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];                 // [2][keys, values]
+  extern __shared__ __attribute__((aligned(1024))) char smem[];                 // keys [2], values [2], what `clean` notes
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
   const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
   RowTile t;
@@ -423,34 +423,38 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
   }
   const int vc = VI::chunk(lane >> 3, lane & 7);           // chunk of an even piece; of an odd one: vc ^ 4
   const int64_t vrow = (int64_t)(lane >> 3) << (a.ix.page_log2 + 1);
-  auto issue = [&](int ti, int buf, int ids) {
-    char* kimg = smem + buf * 2 * IMG;
-    const int base = ti * KT, slot0 = base & pmask;
+  const int voff0 = vc * 16, voff1 = (vc ^ 4) * 16;        // pages of 64 slots or more hold a tile's keys in one piece
+  auto issue_k = [&](int i, int ti, int ids) __attribute__((always_inline)) {      // this wave's piece i of a key image
+    const int piece = i * NW + w, grp = piece * 4 / NC;    // the 16-key group
+    if (NC % NW == 0 || piece < NC) {
+      int id = __builtin_amdgcn_readlane(ids, grp);
+      id = id < 0 ? 0 : id;
+      const char* src = kpool + (((((int64_t)id * a.hkv + kvh) << a.ix.page_log2) + ((ti * KT + 16 * grp) & pmask)) * dh) * 2;
+      load_to_lds(src + koff[i], smem + (ti & 1) * IMG + piece * 1024);
+    }
+  };
+  const char* vsrc[2];                                     // where the value pieces of the next tile come from
+  auto aim_v = [&](int ti, int ids) __attribute__((always_inline)) {
+    if (page >= 64) {
+      int id = __builtin_amdgcn_readlane(ids, 0);
+      id = id < 0 ? 0 : id;
+      const char* at = vpool + (((((int64_t)id * a.hkv + kvh) * dh) << a.ix.page_log2) + ((ti * KT) & pmask)) * 2;
+      vsrc[0] = at + vrow + voff0;
+      vsrc[1] = at + vrow + voff1;
+    } else {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int piece = i * NW + w;
-      if (NC % NW == 0 || piece < NC) {
-        const int grp = piece * 4 / NC;                    // the 16-key group
-        int id = __builtin_amdgcn_readlane(ids, grp);
+      for (int o = 0; o < 2; ++o) {
+        const int c = vc ^ (4 * o);
+        int id = __shfl(ids, c >> 1, 64);
         id = id < 0 ? 0 : id;
-        const char* src = kpool + (((((int64_t)id * a.hkv + kvh) << a.ix.page_log2) + slot0 + ((16 * grp) & pmask)) * dh) * 2;
-        load_to_lds(src + koff[i], kimg + piece * 1024);
+        vsrc[o] = vpool + (((((int64_t)id * a.hkv + kvh) * dh) << a.ix.page_log2) + ((8 * c) & pmask)) * 2 + vrow;
       }
     }
-    const char* vsrc[2];
-#pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int c = vc ^ (4 * o);
-      int id = __shfl(ids, c >> 1, 64);
-      id = id < 0 ? 0 : id;
-      vsrc[o] = vpool + (((((int64_t)id * a.hkv + kvh) * dh) << a.ix.page_log2) + slot0 + ((8 * c) & pmask)) * 2 + vrow;
-    }
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int piece = i * NW + w;
-      if ((NC % NW == 0 || piece < NC) && (EXACT || piece * 8 < dh))
-        load_to_lds(vsrc[piece & 1] + ((int64_t)piece << (a.ix.page_log2 + 4)), kimg + IMG + piece * 1024);
-    }
+  };
+  auto issue_v = [&](int i, int ti) __attribute__((always_inline)) {
+    const int piece = i * NW + w;
+    if ((NC % NW == 0 || piece < NC) && (EXACT || piece * 8 < dh))
+      load_to_lds(vsrc[piece & 1] + ((int64_t)piece << (a.ix.page_log2 + 4)), smem + (2 + (ti & 1)) * IMG + piece * 1024);
   };
 
   f32x16 acc[ND];
@@ -459,51 +463,36 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
   float mx = -INFINITY, l = 0.f;      // maximum in units of log2, sum of this lane's half
-
-  auto compute = [&](int ti, int buf, int ids, bool full) __attribute__((always_inline)) {
-    const char* kimg = smem + buf * 2 * IMG;
-    const char* vimg = kimg + IMG;
-    const int base = ti * KT;
-    int mm = m;
-    asm volatile("" : "+v"(mm));                           // image addresses are made here, not kept over the loop
-    mm &= 31;
-    auto keys = [&](int b, int st) {
-      bf16x8 k = *reinterpret_cast<const bf16x8*>(kimg + 32 * b * NC * 16 + (mm * NC + KI::place(KI::XOR ? mm : 32 * b + mm, 2 * st + h)) * 16);
-      if (!EXACT && 16 * st + 8 * h >= dh) k = bf16x8{};
-      return k;
-    };
-    f32x16 s[2];
+  auto okay_of = [&](int ids) { return (unsigned)(__ballot(ids >= 0) & 0xf); };
+  auto full_of = [&](int ti, unsigned okay) { return ti * KT + KT <= w_min && okay == 0xf; };
+  auto key_of = [&](int ti, int b, int st, int mm) __attribute__((always_inline)) {
+    const char* img = smem + (ti & 1) * IMG;
+    bf16x8 k = *reinterpret_cast<const bf16x8*>(img + 32 * b * NC * 16 + (mm * NC + KI::place(KI::XOR ? mm : 32 * b + mm, 2 * st + h)) * 16);
+    if (!EXACT && 16 * st + 8 * h >= dh) k = bf16x8{};
+    return k;
+  };
+  auto value_of = [&](int ti, int ks, int d, int mm) __attribute__((always_inline)) {
+    return *reinterpret_cast<const bf16x8*>(smem + (2 + (ti & 1)) * IMG + 32 * d * 128 + (mm * 8 + VI::place(mm, 2 * ks + h)) * 16);
+  };
+  auto mask = [&](int ti, unsigned okay, f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int st = 0; st < STEPS; ++st) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(b, st), qf[st], st ? s[b] : f32x16{}, 0, 0, 0);
-    // reads four ahead of the products
-    if constexpr (EXACT) {
-      __builtin_amdgcn_sched_group_barrier(SG_READ, 4, 0);
-#pragma unroll
-      for (int i = 0; i < 2 * STEPS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-        if (i + 4 < 2 * STEPS) __builtin_amdgcn_sched_group_barrier(SG_READ, 1, 0);
+      for (int i = 0; i < 16; ++i) {
+        const int key = 32 * b + 16 * (i >> 3) + 8 * h + (i & 7);
+        if (ti * KT + key >= vis || !(okay >> (2 * b + (i >> 3)) & 1)) s[b][i] = -INFINITY;
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    unsigned okay = 0xf;
-    if (!full) {
-      okay = (unsigned)(__ballot(ids >= 0) & 0xf);
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = 32 * b + 16 * (i >> 3) + 8 * h + (i & 7);
-          if (base + key >= vis || !(okay >> (2 * b + (i >> 3)) & 1)) s[b][i] = -INFINITY;
-        }
-    }
+  };
+  auto max_of = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
     float tm = s[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) tm = fmaxf(tm, s[i >> 4][i & 15]);
+    return tm;
+  };
+  // The maximum moves only when it has grown by 8 (a factor of 256 in the weights, which fp32 sums and bf16 weights hold as
+  // well as 1): the accumulators are rescaled a few times a row instead of every tile.
+  auto raise_max = [&](float tm) __attribute__((always_inline)) {
     tm = fmaxf(tm, __shfl_xor(tm, 32, 64)) * c_abs;
-    // the maximum moves only when it has grown by 8 (a factor of 256 in the weights, which fp32 sums and bf16 weights hold
-    // as well as 1): the accumulators are rescaled a few times a row instead of every tile
     if (__any(tm > mx + 8.f || (mx == -INFINITY && tm > -INFINITY))) {
       const float mn = fmaxf(mx, tm), al = fast_exp2(mx - safe_max(mn));
       l *= al;
@@ -511,96 +500,157 @@ __global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(P
       for (int d = 0; d < ND; ++d) acc[d] *= al;
       mx = mn;
     }
-    const float mu = safe_max(mx);
-    float sum = 0.f;
-    auto weights = [&](int ks) {
-      bf16x8 p;
+  };
+  auto weight = [&](const f32x16 (&s)[2], int i, float mu, float& sum, bf16x8 (&p)[4]) __attribute__((always_inline)) {
+    const float pe = fast_exp2(fmaf(s[i >> 4][i & 15], c_abs, -mu));
+    sum += pe;
+    p[i >> 3][i & 7] = (bf16_t)pe;         // rounded for the second product only, as in the other kernel
+  };
+
+  // Software pipeline, a tile t at a time: the first product of tile t + 1 runs while the vector unit makes the weights of
+  // tile t, the second product of t while it finds the maximum of t + 1.  Keys are loaded two tiles ahead, values one.
+  const int t1w = (w_end + KT - 1) / KT < t1 ? (w_end + KT - 1) / KT : t1;      // the wave's own end
+  int id0 = pages_of(t0), id1 = pages_of(t0 + 1), id2 = pages_of(t0 + 2);
+  f32x16 s[2];
+  if (tid == 0) *reinterpret_cast<volatile int*>(smem + 4 * IMG + 16 * DH) = 0;
+  if (t0 < t1) {
+    aim_v(t0, id0);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      issue_k(i, t0, id0);
+      issue_v(i, t0);
+      if (t0 + 1 < t1) issue_k(i, t0 + 1, id1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t0 < t1w) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_of(t0, b, st, m), qf[st], st ? s[b] : f32x16{}, 0, 0, 0);
+      const unsigned okay = okay_of(id0);
+      if (!full_of(t0, okay)) mask(t0, okay, s);
+      raise_max(max_of(s));
+    }
+  }
+  // Values in a tile that some rows see only in part: slots nobody sees - unwritten ones, a refused page's - may hold anything
+  // and become 0, and so do values that are not finite, whose product with a weight of 0 would be NaN; those are noted by
+  // column and key and added to the rows that see them.
+  uint8_t* noted = reinterpret_cast<uint8_t*>(smem + 4 * IMG);         // [+inf or NaN, -inf or NaN][column][key / 8]: a bit a key
+  volatile int* noted_tile = reinterpret_cast<volatile int*>(smem + 4 * IMG + 16 * DH);
+  auto clean = [&](int ti, unsigned okay) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int n = tid; n < DH * 8; n += NW * 64) {
+      const int dim = n >> 3, c = VI::chunk(dim, n & 7), key = ti * KT + 8 * c;
+      bf16x8* at = reinterpret_cast<bf16x8*>(smem + (2 + (ti & 1)) * IMG) + n;
+      bf16x8 v = *at;
+      unsigned up = 0, down = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float pe = fast_exp2(fmaf(s[ks >> 1][8 * (ks & 1) + e], c_abs, -mu));
-        sum += pe;
-        p[e] = (bf16_t)pe;                 // rounded for the second product only, as in the other kernel
-      }
-      return p;
-    };
-    auto values = [&](int ks, int d) {
-      return *reinterpret_cast<const bf16x8*>(vimg + 32 * d * 128 + (mm * 8 + VI::place(mm, 2 * ks + h)) * 16);
-    };
-    if (full) {
-      // sixteen keys at a time: their products run while the vector unit makes the weights of the next sixteen
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const bf16x8 p = weights(ks);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(ks, d), p, acc[d], 0, 0, 0);
-      }
-      if constexpr (DH <= 192) {
-        __builtin_amdgcn_sched_group_barrier(SG_READ, ND < 4 ? ND : 4, 0);
-        __builtin_amdgcn_sched_group_barrier(SG_VALU, 28, 0);
-#pragma unroll
-        for (int i = 0; i < 4 * ND; ++i) {
-          __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(SG_READ, 1, 0);
-          if (i < 3 * ND) __builtin_amdgcn_sched_group_barrier(SG_VALU, (28 + ND - 1) / ND, 0);
+        const float x = (float)v[e];
+        if (!(okay >> (c >> 1) & 1) || key + e >= t.kv_end || (!EXACT && dim >= dh)) v[e] = (bf16_t)0.f;
+        else if (!(fabsf(x) <= 3.4028235e38f) && key + e >= t.min_vis) {
+          up |= x < INFINITY ? 0u : 1u << e;
+          down |= x > -INFINITY ? 0u : 1u << e;
+          v[e] = (bf16_t)0.f;
         }
       }
+      *at = v;
+      noted[dim * 8 + c] = (uint8_t)up;
+      noted[(DH + dim) * 8 + c] = (uint8_t)down;
+      if (up | down) *noted_tile = ti + 1;
+    }
+  };
+  for (int ti = t0; ti < t1; ++ti) {
+    if (ti > t0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of keys ti + 1 and values ti have landed
+    __syncthreads();                                                   // everyone's have, and everyone has left the buffers of ti - 1
+    const bool next = ti + 1 < t1, after = ti + 2 < t1;
+    if (next) aim_v(ti + 1, id1);
+    const int id3 = pages_of(ti + 3);
+    const unsigned okay = okay_of(id0);
+    const bool part = ti * KT + KT > t.min_vis || okay != 0xf;         // the same for the whole workgroup
+    if (part) {
+      clean(ti, okay);
+      __syncthreads();
+    }
+    if (ti < t1w) {
+      int mm = m;
+      asm volatile("" : "+v"(mm));                         // image addresses are made here, not kept over the loop
+      mm &= 31;
+      const float mu = safe_max(mx);
+      bf16x8 p[4];
+      float sum = 0.f;
       __builtin_amdgcn_sched_barrier(0);
-    } else {
+      // (of no use after the wave's last tile)
+      f32x16 n[2];
+      {
+        constexpr int N = 2 * STEPS;
+        bf16x8 k[AHEAD];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const int k0 = base + 16 * ks + 8 * h;
-        const bool ok = okay >> ks & 1;
-        const bf16x8 p = weights(ks);
-        bf16x8 seen;
+        for (int i = 0; i < AHEAD; ++i) k[i] = key_of(ti + 1, i / STEPS, i % STEPS, mm);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) seen[e] = (bf16_t)(ok && k0 + e < vis ? 1.f : 0.f);
+        for (int i = 0; i < N; ++i) {
+          n[i / STEPS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i % AHEAD], qf[i % STEPS], i % STEPS ? n[i / STEPS] : f32x16{}, 0, 0, 0);
+          if (i + AHEAD < N) k[i % AHEAD] = key_of(ti + 1, (i + AHEAD) / STEPS, (i + AHEAD) % STEPS, mm);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          bf16x8 v = values(ks, d);
-          bool odd = false;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            // slots no row sees - unwritten ones, a refused page's - may hold anything, NaN too
-            if (!ok || k0 + e >= t.kv_end || (!EXACT && 32 * d + mm >= dh)) v[e] = (bf16_t)0.f;
-            odd |= !(fabsf((float)v[e]) <= 3.4028235e38f);
-          }
-          if (__any(odd)) {      // see the other kernel
-            bf16x8 up, down;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = (float)v[e];
-              up[e] = (bf16_t)(x < INFINITY ? 0.f : 1.f);
-              down[e] = (bf16_t)(x > -INFINITY ? 0.f : 1.f);
-              if (!(fabsf(x) <= 3.4028235e38f)) v[e] = (bf16_t)0.f;
-            }
-            const f32x16 nu = __builtin_amdgcn_mfma_f32_32x32x16_bf16(up, seen, f32x16{}, 0, 0, 0);
-            const f32x16 nd = __builtin_amdgcn_mfma_f32_32x32x16_bf16(down, seen, f32x16{}, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (nu[i] > 0.f) acc[d][i] += INFINITY;
-              if (nd[i] > 0.f) acc[d][i] -= INFINITY;
-            }
-          }
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p, acc[d], 0, 0, 0);
+          for (int e = 32 * i / N; e < 32 * (i + 1) / N; ++e) weight(s, e, mu, sum, p);
+          // a load's way into the memory pipe takes as long as some of these steps: they are spread over them
+          if (i * NP / N != (i + 1) * NP / N && after) issue_k(i * NP / N, ti + 2, id2);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      // made here, beside the products, and not where they are used
+      asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]), "+v"(sum));
+      l += sum;
+      s[0] = n[0];
+      s[1] = n[1];
+      const unsigned ok1 = okay_of(id1);
+      if (!full_of(ti + 1, ok1)) mask(ti + 1, ok1, s);
+      __builtin_amdgcn_sched_barrier(0);
+      float tm = s[0][0];
+      {
+        constexpr int N = 4 * ND;
+        bf16x8 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) v[i] = value_of(ti, i / ND, i % ND, mm);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          acc[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[i % AHEAD], p[i / ND], acc[i % ND], 0, 0, 0);
+          if (i + AHEAD < N) v[i % AHEAD] = value_of(ti, (i + AHEAD) / ND, (i + AHEAD) % ND, mm);
+#pragma unroll
+          for (int e = 32 * i / N; e < 32 * (i + 1) / N; ++e) tm = fmaxf(tm, s[e >> 4][e & 15]);
+          if (i * NP / N != (i + 1) * NP / N && next) issue_v(i * NP / N, ti + 1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      asm volatile("" : "+v"(tm));
+      if (part && *noted_tile == ti + 1) {
+        uint64_t sees = 0;
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          if (ti * KT + k < vis && (okay >> (k >> 4) & 1)) sees |= 1ull << k;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int dim = 32 * d + (i & 3) + 8 * (i >> 2) + 4 * h;
+            if (*reinterpret_cast<const uint64_t*>(noted + dim * 8) & sees) acc[d][i] += INFINITY;
+            if (*reinterpret_cast<const uint64_t*>(noted + (DH + dim) * 8) & sees) acc[d][i] -= INFINITY;
+          }
+      }
+      if (ti + 1 < t1w) raise_max(tm);
+    } else {                                               // this wave's rows see no more, but others' do
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (after) issue_k(i, ti + 2, id2);
+        if (next) issue_v(i, ti + 1);
+      }
     }
-    l += sum;
-  };
-
-  int ids = pages_of(t0);
-  if (t0 < t1) issue(t0, 0, ids);
-  for (int ti = t0; ti < t1; ++ti) {
-    const int buf = (ti - t0) & 1, next = pages_of(ti + 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of the tile have landed
-    __syncthreads();                                      // everyone's have, and everyone has left the other buffer
-    if (ti + 1 < t1) issue(ti + 1, buf ^ 1, next);
-    const int base = ti * KT;
-    if (base < w_end) {
-      compute(ti, buf, ids, base + KT <= w_min && (__ballot(ids >= 0) & 0xf) == 0xf);
-    }
-    ids = next;
+    id0 = id1;
+    id1 = id2;
+    id2 = id3;
   }
   l += __shfl_xor(l, 32, 64);
   if (!valid) return;
@@ -754,7 +804,7 @@ extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_
 }
 
 template <int DH, int NW> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
-  constexpr int LDS = 2 * 2 * 64 * DH * 2;
+  constexpr int LDS = 2 * 2 * 64 * DH * 2 + 16 * DH + 16;
   auto kernel = a.dh == DH ? paged_attn_tiles<DH, true, NW> : paged_attn_tiles<DH, false, NW>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
