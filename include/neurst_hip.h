@@ -424,8 +424,8 @@ int neurst_rotary(const void* x, void* y, const double* freq, const int32_t* pos
  * sequence b owns rows cu_new[b] .. cu_new[b + 1] - 1 (none is fine); ctx_len int32 [batch] = tokens in its cache WITH them, so
  * its row j stands at position ctx_len[b] - n_b + j.  Rows of no sequence are left as they are.
  *
- * These arrays live on the device.  A kernel that finds lengths that do not fit (rows out of range, ctx_len < n_b or
- * beyond the table) or a page id outside the pool leaves that sequence or those keys out, and ors 2 or 1 into *status (may
+ * These arrays live on the device.  A kernel that finds lengths that do not fit (rows out of range, ctx_len beyond the
+ * table, or below n_b unless attention is not causal) or a page id outside the pool leaves that sequence or those keys out, and ors 2 or 1 into *status (may
  * be NULL); it reads and writes nothing out of range.
  *
  * neurst_paged_append writes the new keys k (rotated by position when freq is not NULL: pairs, layout, mscale as above) and

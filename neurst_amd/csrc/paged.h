@@ -39,10 +39,11 @@ __device__ __forceinline__ void paged_report(int32_t* status, int bits) {
   NEURST_CHECK_ARG(dh > 0 && dh <= 256 && dh % 8 == 0, name ": dh must be a multiple of 8 up to 256")
 
 static inline PagedIndex paged_index(const int32_t* table, const int32_t* cu, const int32_t* ctx, int64_t tokens, int64_t batch, int64_t wide,
-                                     int64_t ld_table, int64_t page_size, int64_t n_pages) {
+                                     int64_t ld_table, int64_t page_size, int64_t n_pages, bool own) {
   PagedIndex x;
   x.table = table; x.cu = cu; x.ctx = ctx; x.tokens = tokens; x.ld_table = ld_table;
   x.batch = (int)batch; x.wide = (int)wide; x.n_pages = (int)n_pages;
+  x.own = own;
   x.page_log2 = 0;
   while (((int64_t)1 << x.page_log2) < page_size) ++x.page_log2;
   return x;

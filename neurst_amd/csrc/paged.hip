@@ -156,7 +156,7 @@ extern "C" int neurst_paged_append(const void* k, const void* v, const void* q, 
   NEURST_CHECK_ARG(align % 16 == 0, "paged_append: pointers and row strides must be 16-byte aligned");
   if (tokens == 0 || batch == 0) return NEURST_OK;
   AppendArgs a;
-  a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages);
+  a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages, true);
   a.k = k; a.v = v; a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.q_out = q_out; a.freq = freq; a.status = status;
   a.ldk = ldk; a.ldv = ldv; a.ldq = ldq; a.ldqo = ldqo;
   a.hkv = (int)kv_heads; a.hq = (int)q_heads; a.dh = (int)dh; a.hg = 1; a.mscale = mscale;

@@ -882,7 +882,7 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   NEURST_CHECK_ARG(align % 16 == 0, "paged_attention: pointers and row strides must be 16-byte aligned");
   if (tokens == 0 || batch == 0) return NEURST_OK;
   PagedAttnArgs a;
-  a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages);
+  a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages, causal != 0);
   a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.o = o; a.status = status;
   a.ws_o = a.ws_ml = nullptr;
   a.order = nullptr;

@@ -24,6 +24,7 @@ struct PagedIndex {
   int64_t tokens;           // N, rows of the packed tensors
   int64_t ld_table;
   int batch, wide, page_log2, n_pages;
+  int own;                  // the new tokens are part of the cache: ctx >= their number
 };
 
 struct PagedSeq {
@@ -34,8 +35,8 @@ struct PagedSeq {
   int32_t cu;     // cu[b] as it is
 };
 
-// Lengths of sequence b.  Rows out of range: the sequence is left out.  A cache shorter than the rows it should hold, or
-// longer than the page table: the rows exist but nothing is visible to them.
+// Lengths of sequence b.  Rows out of range: the sequence is left out.  A cache shorter than the rows it should hold (`own`),
+// or longer than the page table: the rows exist but nothing is visible to them.
 NEURST_HD PagedSeq paged_seq_of(const PagedIndex& x, int32_t begin, int32_t end, int32_t ctx) {
   PagedSeq s;
   s.row0 = begin;
@@ -48,7 +49,7 @@ NEURST_HD PagedSeq paged_seq_of(const PagedIndex& x, int32_t begin, int32_t end,
     return s;
   }
   s.new_tokens = end - begin;
-  if (ctx < s.new_tokens || ctx > ((int64_t)x.wide << x.page_log2)) {
+  if (ctx < (x.own ? s.new_tokens : 0) || ctx > ((int64_t)x.wide << x.page_log2)) {
     s.bad = PAGED_BAD_LENGTH;
     return s;
   }

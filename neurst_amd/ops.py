@@ -349,10 +349,13 @@ def build_decoder_input(labels, len_labels, sos):
     return inp
 
 
-def embedding_fwd(ids, table, out_dtype, rate, key, pos0=0, signal_len=None, out=None):
+def embedding_fwd(ids, table, out_dtype, rate, key, pos0=0, signal_len=None, out=None, signal=None):
+    """signal: fp32 [Ln, D], the position signal of each column of ids (positions that are not pos0, pos0 + 1, ..)"""
     B, Ln = ids.shape
     V, D = table.shape
-    sig = timing_signal_table(signal_len or (pos0 + Ln), D, ids.device)
+    if signal is not None:
+        assert signal.dtype == torch.float32 and signal.shape == (Ln, D) and pos0 == 0
+    sig = timing_signal_table(signal_len or (pos0 + Ln), D, ids.device) if signal is None else _c(signal)
     if out is None:
         out = torch.empty((B, Ln, D), dtype=torch_dtype(out_dtype), device=ids.device)
     sig_ptr = sig.data_ptr() + pos0 * D * 4

@@ -510,9 +510,15 @@ class TransformerTPE(Seq2SeqModel):
         return self._step(batch)
 
     # ------------------------------------------------------------------ inference (:486-513, :314-325)
-    def infer(self, features, len_feas):
-        """-> (preds [B, steps] int32 numpy, preds_am [B, T] int32 numpy zero padded)."""
+    def infer(self, features, len_feas, prefix=None, len_prefix=None):
+        """-> (preds [B, steps] int32 numpy, preds_am [B, T] int32 numpy zero padded).  With the YAML key `decode: sample` the
+        translations are drawn (Transformer_Decoder.sample_decode; the mapping `sample` has its parameters) and may begin with
+        forced tokens, prefix [B, Lp] and len_prefix [B]; all of them are in self.last['samples']."""
         a = self.args
+        if a.decode not in (None, 'search', 'sample'):
+            raise ValueError("decode must be 'search' (greedy, or beam with beam_size > 1) or 'sample'")
+        if prefix is not None and a.decode != 'sample':
+            raise NotImplementedError("a forced prefix needs decode: sample (with sample.temperature 0 it is the greedy search)")
         if a.dirs and a.dirs.lm_checkpoint:
             raise NotImplementedError('LM rerank (dirs.lm_checkpoint) is outside the hot path')
         beam = (a.beam_size or 1) > 1
@@ -526,7 +532,9 @@ class TransformerTPE(Seq2SeqModel):
             encoded, len_encoded, logits_am, _ = self._encode(feature, len_fea, False, 0.0, batch)
             self.last.update(encoded=encoded, len_encoded=len_encoded)
             with G.variable_scope(self.decoder.name or 'decoder'):
-                if beam:      # TransformerTPE.py:314-319
+                if a.decode == 'sample':
+                    self.last['samples'], preds, len_decoded = self.decoder.sample_decode(encoded, len_encoded, prefix, len_prefix)
+                elif beam:      # TransformerTPE.py:314-319
                     self.last['beams'], preds, len_decoded = self.decoder.beam_decode_rerank(encoded, len_encoded)
                 else:
                     _, preds, len_decoded = self.decoder.decoder_with_caching(encoded, len_encoded)

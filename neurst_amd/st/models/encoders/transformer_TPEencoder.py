@@ -3,6 +3,7 @@ the acoustic encoder without conv / input projection; reads args.model.encoder2.
 from .encoder import Encoder
 from .transformer_encoder import transformer_blocks
 from ..sites import SITE_ENC2_IN, SITE_ENC2_BLK
+from ..tools.utils import Rotary
 from ...layers import common_attention_v1
 
 
@@ -18,5 +19,5 @@ class Transformer_TPEncoder(Encoder):
         bias = common_attention_v1.attention_bias_ignore_padding(len_feas)
         x = common_attention_v1.add_timing_signal_1d(features, dropout_rate=residual_dropout_rate, site=SITE_ENC2_IN)
         x = transformer_blocks(x, bias, len_feas, cfg.num_blocks, cfg.num_cell_units, cfg.num_heads, attention_dropout_rate,
-                               residual_dropout_rate, SITE_ENC2_BLK)
+                               residual_dropout_rate, SITE_ENC2_BLK, rotary=Rotary.of(cfg.rotary, cfg.num_cell_units // cfg.num_heads, x.device))
         return x, len_feas

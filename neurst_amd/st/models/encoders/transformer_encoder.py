@@ -7,12 +7,12 @@ import torch
 from .encoder import Encoder
 from .. import graph as G
 from ..sites import SITE_ENC_IN, SITE_ENC_BLK, blk_site
-from ..tools.utils import residual, multihead_attention, ff_hidden, tf_layers_dense
+from ..tools.utils import Rotary, residual, multihead_attention, ff_hidden, tf_layers_dense
 from ...layers import common_attention_v1, common_layers_v1
 from .... import ops
 
 
-def transformer_blocks(x, bias, len_feas, num_blocks, hidden_units, num_heads, attention_dropout_rate, residual_dropout_rate, site_base):
+def transformer_blocks(x, bias, len_feas, num_blocks, hidden_units, num_heads, attention_dropout_rate, residual_dropout_rate, site_base, rotary=None):
     for i in range(num_blocks):
         with G.variable_scope('block_{}'.format(i)):
             x = residual(x,
@@ -20,7 +20,7 @@ def transformer_blocks(x, bias, len_feas, num_blocks, hidden_units, num_heads, a
                                              total_key_depth=hidden_units, total_value_depth=hidden_units,
                                              output_depth=hidden_units, num_heads=num_heads,
                                              dropout_rate=attention_dropout_rate, name='encoder_self_attention',
-                                             summaries=True, site=blk_site(site_base, i, 0)),
+                                             summaries=True, site=blk_site(site_base, i, 0), rotary=rotary),
                          dropout_rate=residual_dropout_rate, site=blk_site(site_base, i, 1))
             x = residual(x,
                          ff_hidden(inputs=x, hidden_size=4 * hidden_units, output_size=hidden_units, activation='relu'),
@@ -106,5 +106,5 @@ class Transformer_Encoder(Encoder):
                                                      stop_gradient=not has_cnn)
         x = tf_layers_dense(x, hidden_units, use_bias=False, name='encoder_fc', stop_gradient=not has_cnn)
         x = transformer_blocks(x, bias, len_feas, num_blocks, hidden_units, num_heads, attention_dropout_rate, residual_dropout_rate,
-                               SITE_ENC_BLK)
+                               SITE_ENC_BLK, rotary=Rotary.of(args.model.encoder.rotary, hidden_units // num_heads, x.device))
         return x, len_feas

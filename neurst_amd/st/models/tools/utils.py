@@ -43,6 +43,41 @@ _PREGEN_KEEP_BITS = os.environ.get('NEURST_PREGEN_KEEP_BITS', '0') != '0'
 _PREGEN_MIN_WEIGHTS = 1 << 22                                                  # not for decoder-size attention: one more launch costs more than it saves
 
 
+class Rotary:
+    """Rotary positions of a self-attention: the YAML mapping `rotary` of model.encoder / encoder2 / decoder (not in the
+    reference, whose only positions are the added sinusoids of st/layers/common_attention_v1.py:28-70, which stay).  Keys:
+    dims (default: the whole head), base, layout ('half' | 'interleaved') and what ops.rotary_frequencies takes."""
+    _KEYS = {'dims', 'base', 'layout', 'scaling', 'factor', 'original_length', 'turns_fast', 'turns_slow'}
+    _made = {}
+
+    def __init__(self, cfg, dh, device):
+        unknown = set(cfg) - self._KEYS
+        if unknown:
+            raise ValueError('rotary: unknown keys {}'.format(sorted(unknown)))
+        given = {k: v for k, v in cfg.items() if v is not None}
+        self.layout = given.pop('layout', 'half')
+        if self.layout not in ('half', 'interleaved'):
+            raise ValueError('rotary: unknown layout {!r}'.format(self.layout))
+        dims = int(given.pop('dims', dh))
+        if dims > dh:
+            raise ValueError('rotary: dims {} exceeds the head size {}'.format(dims, dh))
+        self.freq, self.mscale = ops.rotary_frequencies(dims, device=device, **given)
+
+    @classmethod
+    def of(cls, cfg, dh, device):
+        """the one for this mapping (None without one), made once"""
+        if not cfg:
+            return None
+        key = (tuple(sorted((k, str(v)) for k, v in cfg.items())), dh, str(device))
+        if key not in cls._made:
+            cls._made[key] = cls(dict(cfg), dh, device)
+        return cls._made[key]
+
+    def turn_(self, x, inverse=False, **where):
+        """in place on x [rows, heads, dh]; where: positions / pos0 / period of ops.rotary"""
+        return ops.rotary(x, self.freq, layout=self.layout, mscale=self.mscale, inverse=inverse, out=x, **where)
+
+
 class BiasGradHook:
     """Set by a dense layer on its output; `residual` marks it taken when it accumulates the bias gradient itself."""
     __slots__ = ('bias', 'taken')
@@ -170,8 +205,9 @@ def residual(inputs, outputs, dropout_rate, site=None, mask_lens=None):
 
 
 def multihead_attention(query_antecedent, memory_antecedent, bias, total_key_depth, total_value_depth, output_depth, num_heads,
-                        dropout_rate, num_queries=None, query_eq_key=False, summaries=False, image_shapes=None, name=None, site=None):
-    """tools/utils.py:479-554.  `bias` is an AttentionBias descriptor or None.  Self-attention runs one
+                        dropout_rate, num_queries=None, query_eq_key=False, summaries=False, image_shapes=None, name=None, site=None, rotary=None):
+    """tools/utils.py:479-554.  `bias` is an AttentionBias descriptor or None.  `rotary` (self-attention only): a Rotary that
+    turns queries and keys by their positions.  Self-attention runs one
     d->3d projection, cross-attention d->d on the queries and d->2d on the memory; q is scaled by
     dh^-0.5, softmax(q k^T + bias), dropout on the weights, . v, heads merged, d->d projection."""
     assert not query_eq_key and num_queries is None, 'only the training forms are routed through this function'
@@ -195,11 +231,16 @@ def multihead_attention(query_antecedent, memory_antecedent, bias, total_key_dep
         if memory_antecedent is None:
             combined = dense(query_antecedent, 3 * d, name='qkv_transform')
             Tk = Tq
+            # the first 2 H of the 3 H heads of a row, turned where they lie; backward turns their gradients back
+            turned = lambda t: t.view(B * Tq, 3 * H, dh)[:, :2 * H]
+            if rotary is not None:
+                rotary.turn_(turned(combined), period=Tq)
             q = (combined, 0, 3 * d)
             k = (combined, d, 3 * d)
             v = (combined, 2 * d, 3 * d)
             qbuf = kvbuf = combined
         else:
+            assert rotary is None, 'rotary positions are for self-attention'
             qbuf = dense(query_antecedent, d, name='q_transform')
             kvbuf = dense(memory_antecedent, 2 * d, name='kv_transform')
             Tk = memory_antecedent.shape[1]
@@ -226,6 +267,8 @@ def multihead_attention(query_antecedent, memory_antecedent, bias, total_key_dep
                     dq, dk, dv = dcomb.view(-1), dcomb.view(-1)[d:], dcomb.view(-1)[2 * d:]
                     ops.mha_bwd(view(q), view(k), view(v), x, dx, lse, dq, dk, dv, q[2], k[2], v[2], 3 * d, 3 * d, 3 * d,
                                 B, H, Tq, Tk, dh, mode, lens, rate, key, keep_bits=kb)
+                    if rotary is not None:
+                        rotary.turn_(turned(dcomb), inverse=True, period=Tq)
                     tape.set(combined, dcomb)
                 else:
                     dqb, dkvb = torch.empty_like(qbuf), torch.empty_like(kvbuf)

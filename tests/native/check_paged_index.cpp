@@ -38,7 +38,7 @@ int main() {
       cu[b + 1] = cu[b] + (n < cap ? n : cap);
       ctx[b] = cu[b + 1] - cu[b] + (int)rnd(cap - (cu[b + 1] - cu[b]) + 1);
     }
-    PagedIndex x = {table.data(), cu.data(), ctx.data(), cu[B] + (int64_t)rnd(30), wide, B, wide, page_log2, 1 + (int)rnd(50)};
+    PagedIndex x = {table.data(), cu.data(), ctx.data(), cu[B] + (int64_t)rnd(30), wide, B, wide, page_log2, 1 + (int)rnd(50), 1};
     for (auto& t : table) t = rnd(x.n_pages);
     if (bad)
       for (int k = 0; k < 12; ++k) {

@@ -262,6 +262,43 @@ def test_paged_attention_long(dtype, new, ctx, hkv, group, dh, page):
 
 
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+def test_contexts_shorter_than_the_chunk(dtype):
+    """not causal: a chunk may be longer than what it attends to (a long prefix against few encoder states), or see nothing"""
+    t, g = TYPES[dtype], gen(59)
+    c = Paged(g, [40, 3, 90, 1], [5, 0, 64, 30], 2, 96, 16, t).put()
+    q = normal(g, c.tokens, 4, 96, dtype=t)
+    want, bound = attend(c, q, False)
+    got = ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=False, status=c.status)
+    within(got, want, bound)
+    assert int(c.status) == 0 and (got[40:43] == 0).all()
+    assert int(c.status) == 0
+    ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=True, status=c.status)
+    assert int(c.status) == 2
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('dh', [32, 64])
+def test_more_workgroups_than_run_at_once(causal, dh):
+    """tiles of rows sorted by their work: ragged chunks of many heads, one sequence without tokens, one of a single token"""
+    t, g = torch.bfloat16, gen(61)
+    new, ctx = [300, 1, 0, 150, 129], [420, 77, 30, 150, 900]
+    c = Paged(g, new, ctx, 40, dh, 32, t, fill=0.0)
+    for b, n in enumerate(ctx):
+        for i in range(-(-n // 32)):
+            m = min(32, n - i * 32)
+            c.k_pages[c.rows[b][i], :, :m] = c.k[b][i * 32:i * 32 + m].transpose(0, 1)
+            c.v_pages[c.rows[b][i], :, :, :m] = c.v[b][i * 32:i * 32 + m].permute(1, 2, 0)
+    q = normal(g, c.tokens + 5, 120, dh, dtype=t)
+    out = torch.full_like(q, 7.0)
+    wide = c.table.shape[1]
+    assert ops.paged_attention_workspace_bytes(c.tokens + 5, 5, wide, 32, 120, 40, dh, lib.BF16) < (c.tokens + 5) * 120 * 4      # the order, no parts
+    ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=causal, out=out, status=c.status)
+    want, bound = attend(c, q[:c.tokens], causal)
+    within(out[:c.tokens], want, bound)
+    assert (out[c.tokens:] == 7.0).all() and int(c.status) == 0
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
 @pytest.mark.parametrize('n,dh', [(40, 64), (200, 96), (300, 128)])
 def test_masked_values_that_are_not_finite(dtype, n, dh):
     """a chunk whose later keys and values are inf and NaN: earlier queries do not see them, later ones do"""
