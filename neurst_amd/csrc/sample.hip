@@ -12,13 +12,14 @@
 // 2^-45 of the best have weight 0 and are never drawn.
 //
 // The kept set is {key > K} and the words with key == K up to a place, keys being the logits in an order-preserving integer
-// form.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in [0, 32) - all that can
+// form.  First the words that can be kept at all are told from a bound (the top_k-th of the threads' own maxima; for top_p how
+// little the tail can weigh; min_p itself) and, up to 1024 of them, listed in index order; the rest of the work runs on that
+// list, a word a thread.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in [0, 32) - all that can
 // have weight - finds the step where the count passes top_k or the sum passes top_p, and the words of that one step, a dozen
-// as a rule, are ranked among each other.  What top_k leaves (up to 1024 words) goes to a list in index order, and the rest of
-// the work runs on that.
+// as a rule, are ranked among each other.
 //
 // One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
-// the chain of passes and barriers for few rows, by the fp64 exponentials (~25 instructions a word) for many without top_k.
+// the chain of passes and barriers, and without top_k by the fp64 exponentials (~20 instructions a word).
 #include "common.h"
 
 struct SampleArgs {
@@ -46,25 +47,38 @@ __device__ __forceinline__ uint32_t logit_key(float l) {
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-// round(2^44 exp(x)), x in [-32, 0]: exp(x) = 2^n exp(y), |y| <= ln2 / 2, Taylor polynomial to y^11 (the next term is 6e-15)
-__device__ __forceinline__ u64 sample_weight(double x) {
-  const double t = x * 1.4426950408889634074, n = rint(t), y = (t - n) * 0.69314718055994530942;
-  double p = 2.50521083854417187751e-08;
-  p = fma(p, y, 2.75573192239858906526e-07);
-  p = fma(p, y, 2.75573192239858906526e-06);
-  p = fma(p, y, 2.48015873015873015873e-05);
-  p = fma(p, y, 1.98412698412698412698e-04);
-  p = fma(p, y, 1.38888888888888888889e-03);
-  p = fma(p, y, 8.33333333333333333333e-03);
-  p = fma(p, y, 4.16666666666666666667e-02);
-  p = fma(p, y, 1.66666666666666666667e-01);
-  p = fma(p, y, 0.5);
-  p = fma(p, y, 1.0);
-  p = fma(p, y, 1.0);
-  // the sum with 2^52 holds the rounded integer in its low 52 bits
-  const double v = ldexp(p, (int)n + 44) + 4503599627370496.0;
-  return __builtin_bit_cast(u64, v) & 0xFFFFFFFFFFFFFull;
-}
+// round(2^44 exp(x)), x in [-32, 0]: exp(x) = 2^(n / 16) exp(y), |y| <= ln2 / 32, with 2^(j / 16) from a table (sixteen values
+// of 2^(j/16), each the double next to it) and the Taylor polynomial to y^6 (the next term is 4e-16).  Its coefficients come
+// in scalar registers: as literals each would cost two moves an evaluation.
+__device__ const double SAMPLE_ROOTS[16] = {
+    1.0, 1.0442737824274138403, 1.0905077326652576592, 1.1387886347566916537, 1.1892071150027210667, 1.2418578120734840486,
+    1.2968395546510096659, 1.3542555469368927283, 1.4142135623730950488, 1.4768261459394993114, 1.5422108254079408236,
+    1.6104903319492543081, 1.6817928305074290861, 1.7562521603732994831, 1.8340080864093424635, 1.9152065613971472939};
+struct SampleExp {
+  double c6, c5, c4, c3;
+  const double* roots;       // in shared memory
+  __device__ __forceinline__ void init(const double* r) {
+    roots = r;
+    c6 = 1.38888888888888888889e-03;
+    c5 = 8.33333333333333333333e-03;
+    c4 = 4.16666666666666666667e-02;
+    c3 = 1.66666666666666666667e-01;
+    asm volatile("" : "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3));
+  }
+  __device__ __forceinline__ u64 operator()(double x) const {
+    const double t = x * 23.083120654223414519, n = rint(t), y = (t - n) * 0.043321698784996581838;
+    const int i = (int)n;
+    double p = fma(c6, y, c5);
+    p = fma(p, y, c4);
+    p = fma(p, y, c3);
+    p = fma(p, y, 0.5);
+    p = fma(p, y, 1.0);
+    p = fma(p, y, 1.0);
+    // the sum with 2^52 holds the rounded integer in its low 52 bits
+    const double v = ldexp(p * roots[i & 15], (i >> 4) + 44) + 4503599627370496.0;
+    return __builtin_bit_cast(u64, v) & 0xFFFFFFFFFFFFFull;
+  }
+};
 
 // ---- 64-lane scans through the DPP network (all lanes active) and sums over the waves of a workgroup ------------------------
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
@@ -97,10 +111,11 @@ template <typename T, int NT> struct SampleShared {
   u64 hw[SAMPLE_BINS];
   SampleCand cand[SAMPLE_CAND];
   u64 ww[2][16], above, bin_w, drawn;
+  double roots[16];
   uint32_t hc[SAMPLE_BINS];
   int list_at[SAMPLE_LIST];
   uint32_t wa[16], wb[16], bin_c, found_key, count;
-  float wf[16];
+  float wf[16], wr[16];      // maxima, sums of roots of the waves
   int bin, found_at, place;
   T list[SAMPLE_LIST];
 };
@@ -115,8 +130,15 @@ template <typename S, int NW> __device__ __forceinline__ void waves_sum(S& s, in
   before = w ? readlane_u64(inc, w - 1) : 0;
 }
 
-// A sequence of words: place i of step and lane, in index order wave by wave, step by step, lane by lane.
-template <typename T, int NT> struct SampleView {
+// NaN is never drawn; -0 counts as +0
+template <typename T> __device__ __forceinline__ float sample_word(T v) {
+  const float x = to_f32<T>(v);
+  return x == x ? x + 0.f : -INFINITY;
+}
+
+// A sequence of words: place i of step and lane, in index order wave by wave, step by step, lane by lane.  CLEAN: in shared
+// memory, gone through sample_word and padded with -inf to whole steps.
+template <typename T, int NT, bool CLEAN> struct SampleView {
   const T* p;                // [n]
   int n, base, steps;
   __device__ __forceinline__ void init(const T* p_, int n_, int tid) {
@@ -126,23 +148,30 @@ template <typename T, int NT> struct SampleView {
     base = (tid >> 6) * steps * 64 + (tid & 63);
   }
   __device__ __forceinline__ float at(int place) const {
-    const float x = place < n ? to_f32<T>(p[place]) : -INFINITY;
-    return x == x ? x + 0.f : -INFINITY;           // NaN is never drawn; -0 counts as +0
+    if constexpr (CLEAN) return to_f32<T>(p[place]);
+    return place < n ? sample_word<T>(p[place]) : -INFINITY;
   }
-  template <int UNROLL = 4, typename F> __device__ __forceinline__ void each(F f) const {
-#pragma unroll UNROLL
-    for (int i = 0; i < steps; ++i) f(at(base + i * 64), base + i * 64);
+  // f(word, place) for this lane's words, four read at a time; past the last step f sees -inf, which has no weight
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    for (int i = 0; i < steps; i += 4) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = i + j < steps ? at(base + (i + j) * 64) : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(v[j], base + (i + j) * 64);
+    }
   }
 };
 
 struct SampleRule {
+  SampleExp exp44;
   float mx, bin_scale;
   double inv_t;
   u64 lowest;                // min_p as a weight
+  // no branch: several words' chains of fp64 instructions run side by side
   __device__ __forceinline__ u64 weight(float l) const {
-    if (l == mx) return (u64)SAMPLE_ONE;
     const double x = ((double)l - (double)mx) * inv_t;
-    return x >= -SAMPLE_SPAN ? sample_weight(x) : 0;
+    return exp44(l == mx ? 0.0 : fmax(x, -(double)SAMPLE_SPAN));       // -32: rounds to 0
   }
   // step of the histogram: grows as l falls, 0 for the best; SAMPLE_BINS: no weight
   __device__ __forceinline__ int step_of(float l) const {
@@ -157,39 +186,49 @@ struct SampleLimit {         // words with key > K, and with key == K up to plac
   __device__ __forceinline__ bool holds(uint32_t key, int place) const { return key > K || (key == K && place <= cut); }
 };
 
-// The word at which the running count (by_weight: the running sum), in descending order, reaches `need`: the new limit.
-// The histogram over the words that `lim` holds is in s.hc / s.hw.
-template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s, const SampleView<T, NT>& r,
-                                                                                                   const SampleRule& rule, SampleLimit lim, u64 need,
-                                                                                                   int tid) {
+// the bin at which the running count (BY_WEIGHT: the running sum) reaches `want`, into s.bin, with what lies before it and in it
+template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ void sample_cross(SampleShared<T, NT>& s, u64 want, int tid) {
   constexpr int NW = NT / 64, PER = SAMPLE_BINS / NT;
   const int lane = tid & 63, w = tid >> 6;
   auto part = [&](int i) -> u64 { return BY_WEIGHT ? s.hw[i] : (u64)s.hc[i]; };
-  // the bin that reaches `need`, into s.bin, with the sum before it and its count
-  auto cross = [&](u64 want) {
-    u64 x = 0;
+  u64 x = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x += part(tid * PER + j);
-    const u64 inc = wave_scan_u64(x);
-    u64 before, all;
-    waves_sum<SampleShared<T, NT>, NW>(s, 1, readlane_u64(inc, 63), w, lane, before, all);
-    u64 b = before + inc - x;
-    if (b < want && b + x >= want) {
-      for (int j = 0; j < PER; ++j) {
-        const u64 y = part(tid * PER + j);
-        if (b + y >= want) {
-          s.bin = tid * PER + j;
-          s.above = b;
-          s.bin_c = s.hc[tid * PER + j];
-          s.bin_w = y;
-          break;
-        }
-        b += y;
+  for (int j = 0; j < PER; ++j) x += part(tid * PER + j);
+  const u64 inc = wave_scan_u64(x);
+  u64 before, all;
+  waves_sum<SampleShared<T, NT>, NW>(s, 1, readlane_u64(inc, 63), w, lane, before, all);
+  u64 b = before + inc - x;
+  if (b < want && b + x >= want) {
+    for (int j = 0; j < PER; ++j) {
+      const u64 y = part(tid * PER + j);
+      if (b + y >= want) {
+        s.bin = tid * PER + j;
+        s.above = b;
+        s.bin_c = s.hc[tid * PER + j];
+        s.bin_w = y;
+        break;
       }
+      b += y;
     }
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-  };
+  }
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+}
+template <typename T, int NT> __device__ __forceinline__ void sample_clear(SampleShared<T, NT>& s, int tid) {
+  __syncthreads();
+  for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
+  __syncthreads();
+}
+
+// The word at which the running count (by_weight: the running sum), in descending order, reaches `need`: the new limit.
+// The histogram over the words that `lim` holds, down to a step behind that word's, is in s.hc / s.hw.
+template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s,
+                                                                                                               const SampleView<T, NT, CLEAN>& r,
+                                                                                                   const SampleRule& rule, SampleLimit lim, u64 need,
+                                                                                                   int tid) {
+  constexpr int NW = NT / 64;
+  const int lane = tid & 63, w = tid >> 6;
+  auto cross = [&](u64 want) { sample_cross<BY_WEIGHT>(s, want, tid); };
   cross(need);
   const int bin = s.bin;
   if (s.bin_c <= SAMPLE_CAND) {
@@ -248,9 +287,7 @@ template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ SampleL
   }
   while (lo < hi) {
     const int bits = 32 - __builtin_clz(hi - lo), shift = bits > 10 ? bits - 10 : 0;      // 1024 bins
-    __syncthreads();
-    for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-    __syncthreads();
+    sample_clear(s, tid);
     r.each([&](float l, int place) {
       const uint32_t k = logit_key(l);
       if (k >= lo && k <= hi && lim.holds(k, place)) {
@@ -277,7 +314,7 @@ template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ SampleL
   waves_sum<SampleShared<T, NT>, NW>(s, 0, readlane_u64(wave_scan_u64(c), 63), w, lane, before, all);
   uint32_t seen = (uint32_t)before;
   if (seen < m)
-    r.template each<1>([&](float l, int place) {
+    r.each([&](float l, int place) {
       const u64 eq = __ballot(logit_key(l) == K);
       const uint32_t here = (uint32_t)__popcll(eq);
       if (seen < m && seen + here >= m && ((eq >> lane) & 1) && seen + (uint32_t)__popcll(eq & ((2ull << lane) - 1)) == m) s.found_at = place;
@@ -287,34 +324,57 @@ template <bool BY_WEIGHT, typename T, int NT> __device__ __forceinline__ SampleL
   return SampleLimit{K, s.found_at};
 }
 
-// top-p and min-p over the words that `lim` holds, and the draw: the place drawn in s.place, its weight in s.drawn; returns
-// the sum of the words kept
-template <typename T, int NT> __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const SampleView<T, NT>& r, const SampleRule& rule,
-                                                                         SampleLimit lim, float top_p, float u, bool fresh, int tid) {
+// top_k, top-p and min-p over a view that holds every word that can be kept, and the draw: the place drawn in s.place, its
+// weight in s.drawn; returns the sum of the words kept.  k: 0 for none.  all: the sum over the row where top_p < 1 and no
+// top_k (the view may lack words), else not read.  Words behind step `far` are not looked at.
+template <typename T, int NT, bool CLEAN> __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const SampleView<T, NT, CLEAN>& r, const SampleRule& rule,
+                                                                         uint32_t k, float top_p, float u, u64 all, int far, int tid) {
   constexpr int NW = NT / 64;
   typedef SampleShared<T, NT> S;
   const int lane = tid & 63, w = tid >> 6;
+  SampleLimit lim = {0u, 0x7fffffff};
   u64 before, total;
-  if (top_p < 1.f) {
-    if (!fresh) {
-      __syncthreads();
-      for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-      __syncthreads();
-    }
-    u64 mine = 0;
-    r.each([&](float l, int place) {
-      const u64 x = lim.holds(logit_key(l), place) ? rule.weight(l) : 0;
-      if (x) {
-        const int b = rule.step_of(l);                       // x != 0: below SAMPLE_BINS
+  if (k) {
+    sample_clear(s, tid);
+    uint32_t mine = 0;
+    r.each([&](float l, int) {
+      const int b = rule.step_of(l);
+      if (b <= far && b < SAMPLE_BINS) {
         atomicAdd(&s.hc[b], 1u);
-        atomicAdd(&s.hw[b], x);
-        mine += x;
+        ++mine;
       }
     });
     waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
+    if (total > (u64)k) lim = sample_select<false>(s, r, rule, lim, (u64)k, tid);      // else every word with weight stays
+  }
+  if (top_p < 1.f) {
+    total = all;
+    if (k) {
+      u64 mine = 0;
+      r.each([&](float l, int place) {
+        const u64 x = rule.weight(l);
+        mine += lim.holds(logit_key(l), place) ? x : 0;
+      });
+      __syncthreads();
+      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
+    }
     u64 need = (u64)ceil((double)top_p * (double)total);
     if (need < 1) need = 1;
-    if (need < total) lim = sample_select<true>(s, r, rule, lim, need, tid);
+    if (need < total) {
+      sample_clear(s, tid);
+      r.each([&](float l, int place) {
+        const int b = rule.step_of(l);
+        if (b <= far && b < SAMPLE_BINS && lim.holds(logit_key(l), place)) {
+          const u64 x = rule.weight(l);
+          if (x) {
+            atomicAdd(&s.hc[b], 1u);
+            atomicAdd(&s.hw[b], x);
+          }
+        }
+      });
+      __syncthreads();
+      lim = sample_select<true>(s, r, rule, lim, need, tid);
+    }
   }
   auto kept = [&](float l, int place) -> u64 {
     const u64 x = lim.holds(logit_key(l), place) ? rule.weight(l) : 0;
@@ -371,7 +431,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   const int64_t row = blockIdx.x;
   extern __shared__ __attribute__((aligned(16))) char row_lds[];
   const T* src = static_cast<const T*>(a.logits) + row * a.ld;
-  SampleView<T, NT> r;
+  SampleView<T, NT, CACHED> r;
   r.init(CACHED ? reinterpret_cast<const T*>(row_lds) : src, a.V, tid);
   float mx = -INFINITY;
   if constexpr (CACHED) {                                   // every lane keeps to its own words: no barrier needed
@@ -379,10 +439,9 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
 #pragma unroll 8
     for (int i = 0; i < r.steps; ++i) {
       const int at = r.base + i * 64;
-      const T x = at < a.V ? src[at] : (T)-INFINITY;
-      dst[at] = x;                                          // the image is padded to whole steps
-      const float l = to_f32<T>(x);
-      mx = l > mx ? l : mx;                                 // not for NaN
+      const float l = at < a.V ? sample_word<T>(src[at]) : -INFINITY;
+      dst[at] = (T)l;                                       // padded to whole steps
+      mx = fmaxf(mx, l);
     }
   } else {
     r.each([&](float l, int) { mx = fmaxf(mx, l); });
@@ -399,8 +458,10 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   float u = a.u[row];
   u = u > 0.f ? (u < 1.f ? u : 1.f) : 0.f;
   for (int i = tid; i < SAMPLE_BINS; i += NT) { s.hc[i] = 0; s.hw[i] = 0; }
-  mx = wave_max(mx) + 0.f;
+  const float own_max = mx;
+  mx = wave_max(mx);
   if (lane == 0) s.wf[w] = mx;
+  if (tid < 16) s.roots[tid] = SAMPLE_ROOTS[tid];
   __syncthreads();
   mx = wave_max(lane < NW ? s.wf[lane] : -INFINITY);
 
@@ -421,51 +482,83 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   } else if (mx > -INFINITY) {
     SampleRule rule;
     rule.mx = mx;
+    rule.exp44.init(s.roots);
     rule.inv_t = 1.0 / (double)temp;
     rule.bin_scale = (float)(SAMPLE_BINS / SAMPLE_SPAN * rule.inv_t);
     rule.lowest = (u64)ceil((double)min_p * SAMPLE_ONE);
-    SampleLimit lim = {0u, 0x7fffffff};
-    bool limited = false;
-    if (top_k < a.V) {
-      uint32_t mine = 0;
+    const bool by_k = top_k < a.V, by_p = top_p < 1.f;
+    u64 before, n, all = 0;
+    // How far down a kept word can lie, as a step of the histogram; as a rule that leaves a few per cent of the words.
+    int far = SAMPLE_BINS;
+    if (min_p > 0.f) {
+      const float steps = (SAMPLE_BINS / SAMPLE_SPAN) * -logf(min_p) + 2.f;
+      far = steps < (float)SAMPLE_BINS ? (int)steps : SAMPLE_BINS;
+    }
+    if (by_k && top_k <= NT) {
+      // the top_k-th of the threads' own maxima bounds the top_k-th of all words
+      const int b = rule.step_of(own_max);
+      if (b < SAMPLE_BINS) atomicAdd(&s.hc[b], 1u);
+      waves_sum<S, NW>(s, 0, (u64)__popcll(__ballot(b < SAMPLE_BINS)), w, lane, before, n);
+      if (n >= (u64)top_k) {
+        sample_cross<false>(s, (u64)top_k, tid);
+        far = s.bin;             // (min_p comes after top_k: its words may be fewer, never others)
+      } else {
+        far = SAMPLE_BINS;
+      }
+    } else if (by_k) {
+      far = SAMPLE_BINS;
+    } else if (by_p) {
+      u64 mine = 0;
+      float roots = 0.f;
+      const float to_half = (float)(0.72134752 * rule.inv_t);            // exp(x / 2) as exp2
       r.each([&](float l, int) {
-        const int b = rule.step_of(l);
-        if (b < SAMPLE_BINS) {
-          atomicAdd(&s.hc[b], 1u);
-          ++mine;
-        }
+        mine += rule.weight(l);
+        roots += l == mx ? 1.f : __builtin_amdgcn_exp2f((l - mx) * to_half);
       });
-      u64 before, n;
-      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, n);
-      limited = n > (u64)top_k;                             // else every word with weight stays
-      if (limited) lim = sample_select<false>(s, r, rule, lim, (u64)top_k, tid);
+      roots = wave_sum(roots);
+      if (lane == 0) s.wr[w] = roots;
+      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, all);
+      // The words behind step `far`, of weight c = e^(-far / 32) at most, weigh sum w <= sqrt(c) sum sqrt(w) together, which must
+      // not exceed what top_p leaves out (a thousandth and two steps to spare for roundings).
+      const float half = wave_sum(lane < NW ? s.wr[lane] : 0.f), rest = (float)((double)all * (1.0 - (double)top_p)) * 5.684341886e-14f;   // 2^-44
+      const float steps = 2.f * (SAMPLE_BINS / SAMPLE_SPAN) * logf(1.001f * half / rest) + 2.f;
+      far = steps < (float)SAMPLE_BINS ? (steps > 0.f ? (int)steps : 0) : SAMPLE_BINS;
+    }
+    n = (u64)a.V;
+    if (far < SAMPLE_BINS) {
+      // They go to a list, in index order, and the rest of the work runs on that.  Told by a logit a step below the bound: more
+      // words do no harm.
+      const float least = fminf(mx, mx - (float)(far + 2) / rule.bin_scale);
+      uint32_t mine = 0;
+      r.each([&](float l, int) { mine += (uint32_t)__popcll(__ballot(l >= least)); });
+      __syncthreads();
+      waves_sum<S, NW>(s, 0, (u64)mine, w, lane, before, n);
+      if (n <= SAMPLE_LIST) {
+        int at = (int)before;
+        r.each([&](float l, int place) {
+          const u64 in = __ballot(l >= least);
+          if (in) {
+            if ((in >> lane) & 1) {
+              const int i = at + __popcll(in & ((1ull << lane) - 1));
+              s.list[i] = (T)l;
+              s.list_at[i] = place;
+            }
+            at += __popcll(in);
+          }
+        });
+        const int padded = ((int)n + NT - 1) / NT * NT;
+        for (int i = (int)n + tid; i < padded; i += NT) s.list[i] = (T)-INFINITY;
+      }
     }
     u64 total;
-    if (limited && top_k <= SAMPLE_LIST) {
-      uint32_t mine = 0;
-      r.each([&](float l, int place) { mine += lim.holds(logit_key(l), place) ? 1u : 0u; });
-      u64 before, n;
+    if (n <= SAMPLE_LIST && far < SAMPLE_BINS) {
       __syncthreads();
-      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, n);
-      int at = (int)before;
-      r.template each<1>([&](float l, int place) {
-        const u64 in = __ballot(lim.holds(logit_key(l), place));
-        if ((in >> lane) & 1) {
-          const int k = at + __popcll(in & ((1ull << lane) - 1));
-          if (k < SAMPLE_LIST) {
-            s.list[k] = (T)l;
-            s.list_at[k] = place;
-          }
-        }
-        at += __popcll(in);
-      });
-      __syncthreads();
-      SampleView<T, NT> few;
+      SampleView<T, NT, true> few;
       few.init(s.list, (int)n, tid);
-      total = sample_draw(s, few, rule, SampleLimit{0u, 0x7fffffff}, top_p, u, false, tid);
+      total = sample_draw(s, few, rule, by_k ? (uint32_t)top_k : 0u, top_p, u, all, SAMPLE_BINS, tid);
       id = s.list_at[s.place];
     } else {
-      total = sample_draw(s, r, rule, lim, top_p, u, top_k >= a.V, tid);
+      total = sample_draw(s, r, rule, by_k ? (uint32_t)top_k : 0u, top_p, u, all, far, tid);
       id = s.place;
     }
     logp = (float)log((double)s.drawn / (double)total);

@@ -687,7 +687,7 @@ def rotary(x, freq, positions=None, pos0=0, period=0, layout='half', mscale=1.0,
     if positions is not None and (positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous()):
         raise ValueError('rotary: positions must be int32 [rows]')
     if out is None:
-        out, ldy = torch.empty((rows, heads, dh), dtype=x.dtype, device=x.device), heads * dh
+        out, ldy = torch.empty_like(x, memory_format=torch.contiguous_format), heads * dh
     else:
         if out.shape != x.shape or out.dtype != x.dtype:
             raise ValueError('rotary: out must have the shape and type of x')
@@ -757,7 +757,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q=None, fr
             raise ValueError('paged_append: q must be [tokens, q_heads, dh] of the type of the keys')
         ldq = _row_stride(q, qh, dh)
         if q_out is None:
-            q_out, ldo = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device), qh * dh
+            q_out, ldo = torch.empty_like(q, memory_format=torch.contiguous_format), qh * dh
         else:
             if q_out.shape != q.shape or q_out.dtype != q.dtype:
                 raise ValueError('paged_append: q_out must have the shape and type of q')
@@ -795,7 +795,7 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_new, ctx_len, scale=None
     if not math.isfinite(scale):
         raise ValueError('paged_attention: scale must be finite')
     if out is None:
-        out, ldo = torch.empty((tokens, qh, dh), dtype=q.dtype, device=q.device), qh * dh
+        out, ldo = torch.empty_like(q, memory_format=torch.contiguous_format), qh * dh
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError('paged_attention: out must have the shape and type of q')
