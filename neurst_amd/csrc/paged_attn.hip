@@ -326,6 +326,8 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+constexpr int TILE_WAVES = 4;      // 32 rows each; two waves took longer at most sizes this kernel is chosen for (32 sequences of 204
+                                   // rows over 8000 keys: 252 against 209 us)
 constexpr int AHEAD = 4;      // fragments read from shared memory ahead of their product
 
 // An image of rows of NC 16-byte chunks: chunk c of row r lies at another place of the row, chosen by r / PER - PER being the
@@ -353,9 +355,9 @@ __device__ __forceinline__ void load_to_lds(const void* src, char* dst) {      /
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
-template <int DH, bool EXACT, int NW>
-__global__ void __launch_bounds__(NW * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(PagedAttnArgs a) {
-  constexpr int ROWS = 32 * NW, KT = 64, NC = DH / 8, STEPS = DH / 16, ND = DH / 32, IMG = KT * DH * 2;
+template <int DH, bool EXACT>
+__global__ void __launch_bounds__(TILE_WAVES * 64, DH <= 128 ? 2 : 1) paged_attn_tiles(PagedAttnArgs a) {
+  constexpr int NW = TILE_WAVES, ROWS = 32 * NW, KT = 64, NC = DH / 8, STEPS = DH / 16, ND = DH / 32, IMG = KT * DH * 2;
   typedef Image<NC> KI;
   typedef Image<8> VI;
   extern __shared__ __attribute__((aligned(1024))) char smem[];                 // keys [2], values [2], what `clean` notes
@@ -764,29 +766,41 @@ static int padded_dh(int64_t dh) {
   return 0;
 }
 
-// What a call launches, from its sizes alone (the lengths are on the device): the kernel by the rows an average sequence
-// brings to a key/value head, and into how many parts the keys are split so that the chip is filled.
+// What a call launches, from its sizes alone (the lengths are on the device): the kernel, and into how many parts the keys are
+// split so that the chip is filled.  Times below are bf16 with causal masks, ragged sequences of up to the stated sizes.
 struct AttnPlan { int tiles, waves, parts, part_keys, order; };
-static int plan_rows(const AttnPlan& p) { return p.tiles ? 32 * p.waves : 16; }
+static int plan_rows(const AttnPlan& p) { return p.tiles ? 32 * TILE_WAVES : 16; }
 static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t page_size, int64_t kv_heads, int64_t group, int64_t dh, int dtype,
                           bool scaled) {
   AttnPlan p;
-  const int64_t rows = cdiv64(tokens, batch) * group, keys = wide * page_size;
-  p.tiles = dtype == NEURST_BF16 && scaled && rows > 32;
-  p.waves = rows > 64 ? 4 : 2;                                  // of 32 rows
+  const int64_t rows = cdiv64(tokens, batch) * group, keys = wide * page_size;      // rows of an average sequence to a key/value head
+  // paged_attn_tiles reads a key once for 128 rows, but a workgroup walks its keys alone; in paged_attn_rows the waves share
+  // them.  So the first needs rows to fill it and work to fill the chip - here from 2/3 G products (rows / tiles in us, 8
+  // key/value heads of 64 columns: 1 x 204 rows x 500 keys 8.6 / 20.7, 8 x 102 x 500 10.4 / 19.9, 32 x 102 x 500 21 / 25,
+  // 1 x 102 x 8000 29 / 26, 32 x 204 x 500 32 / 25, 8 x 204 x 8000 81 / 45, 32 x 25 x 8000 90 / 120, 32 x 409 x 8000 662 / 231)
+  p.tiles = dtype == NEURST_BF16 && scaled && rows > 32 && (double)(batch * kv_heads) * (double)(rows * keys) * (double)dh >= 5.0 * (1 << 27);
   const int64_t wgs = batch * cdiv64(rows, plan_rows(p)) * kv_heads;
-  // parts of equal length, not of equal number a sequence: the workgroups of a ragged batch then take equally long.  A second
-  // launch joins them (4 us), so up to 1024 keys stay whole.
-  const int64_t least = p.tiles ? 1024 : 512, want = p.tiles ? 512 : 4096;
-  int64_t part = cdiv64(cdiv64(keys * wgs, want), least) * least;
+  // Parts of equal length, not of equal number a sequence: the workgroups of a ragged batch then take equally long.  At least
+  // 512 keys each (tiles, 128 rows over 4 x 8000 keys of 128 columns: 45 us, with 1024 keys 58).
+  // Tiles: as many parts as all run at once, two workgroups a CU up to 128 columns, then one.  One part more than that costs a
+  // second turn (3 x 700 rows x 16000 keys: 199 against 152 us; whole, 2 x 1000 x 30000: 945 against 257).
+  // Rows: a second launch joins the parts (4 us), so up to 1024 keys stay whole (4 sequences of one row, 1000 keys: 12.4 us, in
+  // two parts 11.5 and a launch more; 2000 keys: 22 against 13, 16000 keys: 157 against 36); up to 4096 workgroups even out
+  // ragged lengths (32 sequences, 32 heads on 8 of 128 columns, 32000 keys: 476 us, with 512 or 1024 workgroups 560).
+  const int64_t at_once = dh <= 128 ? 512 : 256, least = 512;
+  int64_t part = p.tiles ? cdiv64(keys, wgs < at_once ? at_once / wgs : 1) : cdiv64(keys * wgs, 4096);
+  part = cdiv64(part, p.tiles ? 64 : least) * (p.tiles ? 64 : least);
+  if (part < least) part = least;
   if (part * 64 < keys) part = cdiv64(keys, 64);
   if (part >= keys || keys <= 1024) part = keys;
   p.part_keys = (int)(cdiv64(cdiv64(keys, cdiv64(keys, part)), 64) * 64);
   p.parts = (int)cdiv64(keys, p.part_keys);
-  // few workgroups: eight waves in each
-  if (!p.tiles) p.waves = wgs * p.parts <= 256 ? 8 : 4;
-  // sorted by work where more workgroups are launched than run at once (two a CU)
-  p.order = p.tiles && p.parts == 1 && wgs > 512 && paged_tiles(tokens, batch, group, plan_rows(p), 1) <= (1 << 16);
+  // waves of a row workgroup: eight where few workgroups run (one row, 8 heads of 64 columns, 500 keys: 8 sequences 8.0 us
+  // against 8.4 with four, 32 sequences 10.3 / 11.0; 64 sequences 14.9 / 13.8, 128 sequences 24.8 / 22.4)
+  p.waves = p.tiles ? TILE_WAVES : wgs * p.parts <= 256 ? 8 : 4;
+  // tiles sorted by work where more workgroups are launched than run at once (three sequences of up to 4096 rows over 9000 keys,
+  // 16 heads on 4 of 128 columns: 519 us, as they come 548)
+  p.order = p.tiles && p.parts == 1 && wgs > at_once && paged_tiles(tokens, batch, group, plan_rows(p), 1) <= (1 << 16);
   return p;
 }
 static int64_t plan_bytes(const AttnPlan& p, int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t dh) {
@@ -803,14 +817,14 @@ extern "C" int64_t neurst_paged_attention_workspace_bytes(int64_t tokens, int64_
   return a > b ? a : b;
 }
 
-template <int DH, int NW> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
+template <int DH> static int tiles_launch(const PagedAttnArgs& a, dim3 grid, hipStream_t s) {
   constexpr int LDS = 2 * 2 * 64 * DH * 2 + 16 * DH + 16;
-  auto kernel = a.dh == DH ? paged_attn_tiles<DH, true, NW> : paged_attn_tiles<DH, false, NW>;
+  auto kernel = a.dh == DH ? paged_attn_tiles<DH, true> : paged_attn_tiles<DH, false>;
   if (LDS > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) { neurst_set_error("paged_attention: cannot reserve %d B of LDS: %s", LDS, hipGetErrorString(e)); return NEURST_E_LAUNCH; }
   }
-  kernel<<<grid, NW * 64, LDS, s>>>(a);
+  kernel<<<grid, TILE_WAVES * 64, LDS, s>>>(a);
   return NEURST_OK;
 }
 
@@ -832,12 +846,12 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   if (plan.tiles) {
     if constexpr (sizeof(T) == 2) {
       switch (pd) {
-        case 32: if (int e = plan.waves == 2 ? tiles_launch<32, 2>(a, grid, s) : tiles_launch<32, 4>(a, grid, s)) return e; break;
-        case 64: if (int e = plan.waves == 2 ? tiles_launch<64, 2>(a, grid, s) : tiles_launch<64, 4>(a, grid, s)) return e; break;
-        case 96: if (int e = plan.waves == 2 ? tiles_launch<96, 2>(a, grid, s) : tiles_launch<96, 4>(a, grid, s)) return e; break;
-        case 128: if (int e = plan.waves == 2 ? tiles_launch<128, 2>(a, grid, s) : tiles_launch<128, 4>(a, grid, s)) return e; break;
-        case 192: if (int e = plan.waves == 2 ? tiles_launch<192, 2>(a, grid, s) : tiles_launch<192, 4>(a, grid, s)) return e; break;
-        case 256: if (int e = plan.waves == 2 ? tiles_launch<256, 2>(a, grid, s) : tiles_launch<256, 4>(a, grid, s)) return e; break;
+        case 32: if (int e = tiles_launch<32>(a, grid, s)) return e; break;
+        case 64: if (int e = tiles_launch<64>(a, grid, s)) return e; break;
+        case 96: if (int e = tiles_launch<96>(a, grid, s)) return e; break;
+        case 128: if (int e = tiles_launch<128>(a, grid, s)) return e; break;
+        case 192: if (int e = tiles_launch<192>(a, grid, s)) return e; break;
+        case 256: if (int e = tiles_launch<256>(a, grid, s)) return e; break;
       }
     }
   } else {

@@ -2,8 +2,10 @@
 // are the added sinusoids of st/layers/common_attention_v1.py:28-70; this is the other form of them, applied to the
 // queries and keys of st/models/tools/utils.py:479-554.
 //
-// Bound by memory: 2 * sizeof(T) bytes an element.  A thread computes the angles of its chunk of pairs once and applies
-// them to `hg` heads; neighbouring threads hold neighbouring chunks of a head, so a wave reads whole lines.
+// Bound by memory: 2 * sizeof(T) bytes an element.  A thread turns one 16-byte chunk of one head and its partner;
+// neighbouring threads hold neighbouring chunks of a head, so a wave reads whole lines.  Computing the angles once for four
+// heads a thread was slower at every size but one: the loads of the heads wait for each other (bf16, 16 heads of 96 columns:
+// 512 rows 4.3 against 3.1 us, 4000 rows 7.7 / 7.5, 8000 rows 10.6 / 11.0, 16000 rows 21.3 / 19.2 = 5.1 TB/s).
 #include "rotary.h"
 
 struct RotArgs {
@@ -13,7 +15,7 @@ struct RotArgs {
   const int32_t* pos;
   int64_t ldx, ldy, row0;
   uint32_t rows, period, base;      // base: row0 modulo period
-  int heads, hg, head_groups, pos0;
+  int heads, pos0;
   float mscale, sign;
   RotShape sh;
 };
@@ -21,21 +23,19 @@ struct RotArgs {
 template <typename T, int VEC> __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   const uint32_t c = idx % (uint32_t)a.sh.chunks, rest = idx / (uint32_t)a.sh.chunks;
-  const uint32_t hgi = rest % (uint32_t)a.head_groups, r = rest / (uint32_t)a.head_groups;
+  const uint32_t h = rest % (uint32_t)a.heads, r = rest / (uint32_t)a.heads;
   if (r >= a.rows) return;
   const int64_t row = a.row0 + r;
-  const T* src = static_cast<const T*>(a.x) + row * a.ldx;
-  T* dst = static_cast<T*>(a.y) + row * a.ldy;
-  const int h0 = (int)hgi * a.hg, h1 = h0 + a.hg < a.heads ? h0 + a.hg : a.heads;
+  const T* src = static_cast<const T*>(a.x) + row * a.ldx + (int64_t)h * a.sh.dh;
+  T* dst = static_cast<T*>(a.y) + row * a.ldy + (int64_t)h * a.sh.dh;
   if ((int)c >= a.sh.rot_chunks) {
-    if (src != dst)
-      for (int h = h0; h < h1; ++h) rot_pass<T, VEC>(a.sh, src + h * a.sh.dh, dst + h * a.sh.dh, (int)c);
+    if (src != dst) rot_pass<T, VEC>(a.sh, src, dst, (int)c);
     return;
   }
   const int p = a.pos ? a.pos[row] : a.pos0 + (int)(a.period ? (a.base + r) % a.period : (uint32_t)row);
   float cs[VEC], sn[VEC];
   rot_angles<VEC>(a.sh, a.freq, (int)c, p, a.mscale, a.sign, cs, sn);
-  for (int h = h0; h < h1; ++h) rot_apply<T, VEC>(a.sh, src + h * a.sh.dh, dst + h * a.sh.dh, (int)c, cs, sn);
+  rot_apply<T, VEC>(a.sh, src, dst, (int)c, cs, sn);
 }
 
 template <typename T> static int rotary_launch(RotArgs a, int64_t rows, hipStream_t s) {
@@ -47,12 +47,7 @@ template <typename T> static int rotary_launch(RotArgs a, int64_t rows, hipStrea
   // interleaved pairs that are not aligned to two elements: element-wise vectors of 2 read as T[2] need 2 * es alignment, so
   // such a tensor is refused by the caller's check
   a.sh = rot_shape(a.sh.n, a.sh.dh, a.sh.layout, vec);
-  // heads per thread: the angles (about 30 instructions a pair) are shared by `hg` heads once there are enough rows to fill
-  // the chip without splitting the heads
-  const int64_t per_head = rows * a.sh.chunks;
-  a.hg = per_head * cdiv64(a.heads, 4) >= 256 * 1024 ? 4 : 1;
-  a.head_groups = (int)cdiv64(a.heads, a.hg);
-  const int64_t per_row = (int64_t)a.sh.chunks * a.head_groups;
+  const int64_t per_row = (int64_t)a.sh.chunks * a.heads;
   const int64_t slice = ((int64_t)1 << 31) / per_row;          // the index of a launch fits 32 bits
   for (int64_t r0 = 0; r0 < rows; r0 += slice) {
     a.row0 = r0;

@@ -220,16 +220,40 @@ def attend(c, q, causal=True, scale=None):
     return out, bound + 1e-30
 
 
-@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+def crowded(c, q, how):
+    """(queries, page table) that ask for the same at sizes of many products, where bf16 goes to the kernel for many rows: behind
+    the last sequence more rows of no sequence ('rows': so many that the keys stay whole; 'split': with a table of 4096 keys)"""
+    if not how:
+        return q, c.table
+    (B, wide), (_, hq, dh) = c.table.shape, q.shape
+    table = c.table
+    if how == 'split' and wide * c.page < 4096:
+        table = torch.cat([table, torch.full((B, 4096 // c.page - wide), -1, dtype=torch.int32, device=DEV)], 1)
+    rows = max(-(-(5 << 27) // (hq * table.shape[1] * c.page * dh)) + B, 33 * B)
+    if how == 'rows':
+        rows = max(rows, 512 * 128 * 2)
+    more = torch.ones(max(0, rows - q.shape[0]), hq, dh, dtype=q.dtype, device=DEV)
+    return torch.cat([torch.cat([q, more]).flatten(1), torch.ones(max(rows, q.shape[0]), 64, dtype=q.dtype, device=DEV)], 1)[:, :-64].unflatten(1, (hq, dh)), table
+
+
+FORMS = [('fp32', ''), ('bf16', ''), ('bf16', 'rows'), ('bf16', 'split')]
+
+
+@pytest.mark.parametrize('dtype,how', FORMS)
 @pytest.mark.parametrize('causal', [True, False])
 @pytest.mark.parametrize('lengths', list(LENGTHS))
 @pytest.mark.parametrize('hkv,group,dh,page', [(2, 1, 8, 16), (1, 3, 96, 32), (3, 1, 72, 16), (2, 2, 64, 64), (1, 8, 128, 16), (1, 1, 192, 32),
                                                (1, 5, 256, 16), (2, 1, 32, 128)])
-def test_paged_attention(dtype, causal, lengths, hkv, group, dh, page):
+def test_paged_attention(dtype, how, causal, lengths, hkv, group, dh, page):
     t, g = TYPES[dtype], gen(11)
     new, ctx = LENGTHS[lengths]
     c = Paged(g, new, ctx, hkv, dh, page, t).put()
-    q = normal(g, c.tokens + 3, hkv * group, dh, dtype=t)
+    q, c.table = crowded(c, normal(g, c.tokens + 3, hkv * group, dh, dtype=t), how)
+    need = ops.paged_attention_workspace_bytes(q.shape[0], *c.table.shape, page, hkv * group, hkv, dh, ops.dt_of(q))
+    if how == 'rows':
+        assert 0 < need < 65536 * 4             # the order of the tiles, no parts
+    elif how == 'split':
+        assert need >= 2 * q.shape[0] * hkv * group * dh * 4
     out = torch.full_like(q, 7.0)
     ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=causal, out=out, status=c.status)
     want, bound = attend(c, q[:c.tokens], causal)
@@ -238,12 +262,12 @@ def test_paged_attention(dtype, causal, lengths, hkv, group, dh, page):
     assert (out[c.tokens:] == 7.0).all()
 
 
-@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+@pytest.mark.parametrize('dtype,how', FORMS)
 @pytest.mark.parametrize('new,ctx,hkv,group,dh,page', [([1, 1, 1], [3001, 17, 4096], 2, 4, 64, 16), ([1], [20000], 1, 1, 128, 64),
                                                        ([300, 1, 129], [1500, 900, 129], 2, 2, 64, 32), ([257, 700], [257, 1000], 1, 4, 128, 16),
                                                        ([1000], [1000], 2, 1, 96, 64), ([520, 3], [520, 2000], 1, 2, 192, 64),
                                                        ([260, 40], [300, 40], 1, 3, 256, 32), ([150] * 4, [333] * 4, 2, 1, 40, 16)])
-def test_paged_attention_long(dtype, new, ctx, hkv, group, dh, page):
+def test_paged_attention_long(dtype, how, new, ctx, hkv, group, dh, page):
     """split contexts and chunks of many rows"""
     t, g = TYPES[dtype], gen(13)
     c = Paged(g, new, ctx, hkv, dh, page, t, fill=0.0)
@@ -254,24 +278,25 @@ def test_paged_attention_long(dtype, new, ctx, hkv, group, dh, page):
             c.v_pages[c.rows[b][i], :, :, :m] = c.v[b][i * page:i * page + m].permute(1, 2, 0)
     packed = normal(g, c.tokens, hkv * group * dh + 64, dtype=t)
     q = packed[:, 64:].unflatten(1, (-1, dh))
+    many, c.table = crowded(c, q, how)
     for causal in (True, False):
         want, bound = attend(c, q, causal)
-        within(ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=causal), want, bound, 'causal %s' % causal)
+        within(ops.paged_attention(many, c.k_pages, c.v_pages, *c.index(), causal=causal)[:c.tokens], want, bound, 'causal %s' % causal)
     want, bound = attend(c, q, True, -0.3)
-    within(ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), scale=-0.3), want, bound, 'scale')
+    within(ops.paged_attention(many, c.k_pages, c.v_pages, *c.index(), scale=-0.3)[:c.tokens], want, bound, 'scale')
 
 
-@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
-def test_contexts_shorter_than_the_chunk(dtype):
+@pytest.mark.parametrize('dtype,how', FORMS)
+def test_contexts_shorter_than_the_chunk(dtype, how):
     """not causal: a chunk may be longer than what it attends to (a long prefix against few encoder states), or see nothing"""
     t, g = TYPES[dtype], gen(59)
     c = Paged(g, [40, 3, 90, 1], [5, 0, 64, 30], 2, 96, 16, t).put()
     q = normal(g, c.tokens, 4, 96, dtype=t)
     want, bound = attend(c, q, False)
+    q, c.table = crowded(c, q, how)
     got = ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=False, status=c.status)
-    within(got, want, bound)
+    within(got[:c.tokens], want, bound)
     assert int(c.status) == 0 and (got[40:43] == 0).all()
-    assert int(c.status) == 0
     ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), causal=True, status=c.status)
     assert int(c.status) == 2
 
@@ -298,9 +323,9 @@ def test_more_workgroups_than_run_at_once(causal, dh):
     assert (out[c.tokens:] == 7.0).all() and int(c.status) == 0
 
 
-@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+@pytest.mark.parametrize('dtype,how', FORMS)
 @pytest.mark.parametrize('n,dh', [(40, 64), (200, 96), (300, 128)])
-def test_masked_values_that_are_not_finite(dtype, n, dh):
+def test_masked_values_that_are_not_finite(dtype, how, n, dh):
     """a chunk whose later keys and values are inf and NaN: earlier queries do not see them, later ones do"""
     t, g = TYPES[dtype], gen(17)
     c = Paged(g, [n], [n + 20], 2, dh, 16, t)
@@ -311,7 +336,8 @@ def test_masked_values_that_are_not_finite(dtype, n, dh):
     c.k[0][first + 1] = float('nan')
     c.put()
     q = normal(g, n, 2, dh, dtype=t)
-    got = ops.paged_attention(q, c.k_pages, c.v_pages, *c.index())
+    many, c.table = crowded(c, q, how)
+    got = ops.paged_attention(many, c.k_pages, c.v_pages, *c.index())[:n]
     c.k, c.v = clean
     want, bound = attend(c, q)
     cut = n // 2
@@ -339,29 +365,30 @@ def test_pages_shared_by_sequences():
     within(ops.paged_attention(q[:1], c.k_pages, c.v_pages, one, i32([0, 1]), i32([64])), want, bound)
 
 
-@pytest.mark.parametrize('n', [1, 40, 200])
-def test_bad_pages_and_lengths_are_left_out(n):
+@pytest.mark.parametrize('n,how', [(1, ''), (40, ''), (200, ''), (1, 'rows'), (40, 'rows'), (200, 'rows'), (40, 'split'), (200, 'split')])
+def test_bad_pages_and_lengths_are_left_out(n, how):
     """the index arithmetic's own test runs on the CPU; here the kernels keep to it and report"""
     t, g = torch.bfloat16, gen(23)
     hkv, dh, page = 2, 64, 16
     c = Paged(g, [n, n, n], [n + 40, n + 40, n + 40], hkv, dh, page, t).put()
     q = normal(g, 3 * n, hkv, dh, dtype=t)
-    good = ops.paged_attention(q, c.k_pages, c.v_pages, *c.index(), status=c.status)
+    many, c.table = crowded(c, q, how)
+    good = ops.paged_attention(many, c.k_pages, c.v_pages, *c.index(), status=c.status)
     ops.paged_check(c.status)
     table = c.table.clone()
     table[1, 1] = 10 ** 6
-    got = ops.paged_attention(q, c.k_pages, c.v_pages, table, c.cu, c.ctx_len, status=c.status)
-    assert int(c.status) == 1 and torch.equal(got[:n], good[:n]) and torch.equal(got[2 * n:], good[2 * n:])
+    got = ops.paged_attention(many, c.k_pages, c.v_pages, table, c.cu, c.ctx_len, status=c.status)
+    assert int(c.status) == 1 and torch.equal(got[:n], good[:n]) and torch.equal(got[2 * n:3 * n], good[2 * n:3 * n])
     d = Paged(g, [n], [n + 40 - page], hkv, dh, page, t)         # the same without the page's keys: later queries, not causal
     d.k, d.v = [torch.cat([c.k[1][:page], c.k[1][2 * page:]])], [torch.cat([c.v[1][:page], c.v[1][2 * page:]])]
     want, bound = attend(d, q[n:2 * n], False)
-    within(ops.paged_attention(q, c.k_pages, c.v_pages, table, c.cu, c.ctx_len, causal=False)[n:2 * n], want, bound)
+    within(ops.paged_attention(many, c.k_pages, c.v_pages, table, c.cu, c.ctx_len, causal=False)[n:2 * n], want, bound)
     with pytest.raises(lib.NeurstLibError, match='page id'):
         ops.paged_check(c.status)
     for ctx in ([n + 40, n - 1, n + 40], [n + 40, 10 ** 9, n + 40], [n + 40, -5, n + 40]):
         c.status.zero_()
-        got = ops.paged_attention(q, c.k_pages, c.v_pages, c.table, c.cu, i32(ctx), status=c.status)
-        assert int(c.status) == 2 and torch.equal(got[:n], good[:n]) and torch.equal(got[2 * n:], good[2 * n:])
+        got = ops.paged_attention(many, c.k_pages, c.v_pages, c.table, c.cu, i32(ctx), status=c.status)
+        assert int(c.status) == 2 and torch.equal(got[:n], good[:n]) and torch.equal(got[2 * n:3 * n], good[2 * n:3 * n])
         assert (got[n:2 * n] == 0).all()
     kp, vp = c.k_pages.clone(), c.v_pages.clone()
     k = normal(g, 3 * n, hkv, dh, dtype=t)
@@ -391,7 +418,10 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(k_pages[n_pages - 1], c.k[0][:64].transpose(0, 1)) and torch.equal(v_pages[n_pages - 7, :, :, :22], c.v[0][128:].permute(1, 2, 0))
     q = normal(g, 70, hkv, dh, dtype=t)
     want, bound = attend(c, q)
-    within(ops.paged_attention(q, k_pages, v_pages, table, c.cu, c.ctx_len), want, bound)
+    for how in ('', 'rows'):
+        c.table = table
+        many, wide = crowded(c, q, how)
+        within(ops.paged_attention(many, k_pages, v_pages, wide, c.cu, c.ctx_len)[:70], want, bound, how)
     del k_pages, v_pages
     torch.cuda.empty_cache()
 
