@@ -7,7 +7,8 @@
 // 16-byte load from the page, with no trip through shared memory.  The price is paid here, once per token: a chunk is
 // transposed in registers eight slots at a time, a single token scatters dh elements of 2 bytes.
 //
-// Bound by memory (chunks) or by the launch (single tokens).  A tile is 64 positions aligned in the cache; its items - 16
+// Bound by memory (chunks: 37 sequences of up to 700 tokens, 8 heads of 64 columns, bf16, 30 us = 3.5 TB/s - the transposition
+// reads and writes 128-byte pieces) or by the launch (64 single tokens of 96 columns: 5.0 us).  A tile is 64 positions aligned in the cache; its items - 16
 // bytes of a query or key row with its partner of the pair, eight slots x eight columns of values - are dealt to
 // gridDim.y workgroups.  Lanes of a value item run over the slot groups first, then over the columns: a wave reads whole
 // 128-byte row pieces and writes whole 128-byte column pieces.
@@ -115,14 +116,16 @@ template <typename T> static int append_launch(AppendArgs a, int64_t pairs, int 
   if (!rot_vec_fits(pairs, a.dh, layout, vec)) vec = layout == ROT_HALF ? 1 : 2;
   a.sh = rot_shape(pairs, a.dh, layout, vec);
   const int64_t tiles = paged_tiles(a.ix.tokens, a.ix.batch, 1, APPEND_TILE, 2);
-  // items of an average sequence's tile decide over how many workgroups a tile is dealt; the angles are shared by four heads
-  // once that leaves a workgroup's worth of items for every CU
+  // items of an average sequence's tile decide over how many workgroups a tile is dealt; the angles are shared by two heads
+  // once two workgroups' worth of items for every CU are there (bf16, 8 + 8 heads of 64 columns, one head / two / four, us:
+  // 64 sequences of one token 4.4 / 5.6 / 6.5, 8 of up to 200 5.7 / 6.3 / 8.0, 37 of up to 60 9.1 / 9.0 / 10.5, of up to 200
+  // 15.0 / 12.6 / 14.7, of up to 700 35.3 / 30.4 / 30.3)
   int64_t per = cdiv64(a.ix.tokens, a.ix.batch);
   if (per > APPEND_TILE) per = APPEND_TILE;
   const int heads = a.hkv + a.hq;
-  a.hg = a.ix.tokens * a.sh.chunks * cdiv64(heads, 4) >= 256 * 256 ? 4 : 1;
+  a.hg = a.ix.tokens * a.sh.chunks * heads >= 2 * 256 * 256 ? 2 : 1;
   const int64_t items = per * a.sh.chunks * cdiv64(heads, a.hg) + cdiv64(per, 16 / es) * (a.dh / (16 / es)) * a.hkv;
-  int64_t gy = cdiv64(items, 256);
+  int64_t gy = cdiv64(items, 256);      // one item a thread (37 sequences of up to 700: 30.5 us; two items 31.9, four 33.6)
   if (gy > 64) gy = 64;
   const dim3 grid((unsigned)tiles, (unsigned)gy);
   switch (vec) {

@@ -14,12 +14,14 @@
 // The kept set is {key > K} and the words with key == K up to a place, keys being the logits in an order-preserving integer
 // form.  First the words that can be kept at all are told from a bound (the top_k-th of the threads' own maxima; for top_p how
 // little the tail can weigh; min_p itself) and, up to 1024 of them, listed in index order; the rest of the work runs on that
-// list, a word a thread.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in [0, 32) - all that can
-// have weight - finds the step where the count passes top_k or the sum passes top_p, and the words of that one step, a dozen
-// as a rule, are ranked among each other.
+// list, a word a thread.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in
+// [0, 32) - all that can have weight - finds the step where the count passes top_k or the sum passes top_p, and the words of
+// that one step, a dozen as a rule, are ranked among each other.  (Without the list every pass ran over the row: the 256 rows
+// below took 86 us.)
 //
 // One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
-// the chain of passes and barriers, and without top_k by the fp64 exponentials (~20 instructions a word).
+// the chain of passes and barriers: one row of 10000 words with top_p takes 17 us, 256 rows of 32003 words with every filter,
+// a CU each, 30 us = 1.1 TB/s.
 #include "common.h"
 
 struct SampleArgs {
