@@ -741,7 +741,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q=None, fr
     of no sequence are undefined; None without q)."""
     dt = dt_of(k)
     n_pages, kvh, page, dh, B, wide, ldt = _paged_index(k_pages, v_pages, page_table, cu_new, ctx_len, status)
-    tokens = k.shape[0]
+    tokens = k.shape[0] if k.dim() == 3 else -1
     if k.shape != (tokens, kvh, dh) or v.shape != k.shape or k.dtype != k_pages.dtype or v.dtype != k.dtype:
         raise ValueError('paged_append: k and v must be [tokens, kv_heads, dh] of the type of the pages')
     ldk, ldv = _row_stride(k, kvh, dh), _row_stride(v, kvh, dh)
@@ -752,7 +752,7 @@ def paged_append(k, v, k_pages, v_pages, page_table, cu_new, ctx_len, q=None, fr
     pairs = 0 if freq is None else _freq_pairs(freq, dh)
     qh = ldq = ldo = 0
     if q is not None:
-        qh = q.shape[1]
+        qh = q.shape[1] if q.dim() == 3 else -1
         if q.shape != (tokens, qh, dh) or q.dtype != k.dtype:
             raise ValueError('paged_append: q must be [tokens, q_heads, dh] of the type of the keys')
         ldq = _row_stride(q, qh, dh)
@@ -857,7 +857,7 @@ def _sample_args(logits2d, u, values):
             if x.dtype != dt or x.shape != (R,) or not x.is_contiguous() or not _here(logits2d, x):
                 raise ValueError('sample: {} per row must be {} [rows] on the current GPU'.format(what, dt))
             pointers[i], numbers[i] = x.data_ptr(), default
-    numbers[1] = min(int(numbers[1]), 0x7fffffff)
+    numbers[1] = max(min(int(numbers[1]), 0x7fffffff), -1)      # what a C int holds; -1 is refused there
     return R, V, ld, pointers + numbers
 
 

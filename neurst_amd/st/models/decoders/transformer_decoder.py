@@ -168,8 +168,9 @@ class Transformer_Decoder(Decoder):
         get = lambda key, default: default if s.get(key) is None else s[key]
         num = int(get('num', 1))
         rule = dict(temperature=float(get('temperature', 1.0)), top_k=int(get('top_k', 0)), top_p=float(get('top_p', 1.0)), min_p=float(get('min_p', 0.0)))
-        if num < 1:
-            raise ValueError('sample: num must be at least 1')
+        page = int(get('page_size', 16))
+        if num < 1 or page not in [1 << i for i in range(4, 13)]:
+            raise ValueError('sample: num must be at least 1, page_size a power of two in 16..4096')
         B, T = encoded.shape[0], encoded.shape[1]
         R, dev = B * num, encoded.device
         max_steps = int(min(T + 50, self.args.max_len))
@@ -177,12 +178,19 @@ class Transformer_Decoder(Decoder):
         lp = np.zeros(B, np.int64)
         if prefix is not None:
             prefix = host(prefix)
+            if prefix.ndim != 2 or prefix.dtype.kind not in 'iu':
+                raise ValueError('sample: prefix must be whole numbers [batch, length]')
             lp = np.full(B, prefix.shape[1], np.int64) if len_prefix is None else host(len_prefix).astype(np.int64)
             if prefix.shape[0] != B or lp.shape != (B,) or (lp < 0).any() or (lp > prefix.shape[1]).any():
                 raise ValueError('sample: prefix must be [batch, length], len_prefix [batch] within it')
+            held = prefix[np.arange(prefix.shape[1])[None] < lp[:, None]]
+            if (held < 0).any() or (held >= self.dim_output).any():
+                raise ValueError('sample: a token of prefix is not in the vocabulary')
+        elif len_prefix is not None:
+            raise ValueError('sample: len_prefix without prefix')
         first = [np.concatenate([[self.start_token], prefix[b, :lp[b]] if lp[b] else []]).astype(np.int32) for b in range(B) for _ in range(num)]
         lens = np.repeat(lp, num) + 1                                      # tokens of the first chunk
-        run = _PagedDecoderStep(self, encoded, len_encoded, num, lens, max_steps, int(get('page_size', 16)))
+        run = _PagedDecoderStep(self, encoded, len_encoded, num, lens, max_steps, page)
         gen = torch.Generator(device=dev).manual_seed(int(get('seed', self.args.seed or 0)))
         us = torch.rand((max_steps, R), generator=gen, device=dev)
         zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)

@@ -112,6 +112,16 @@ def test_refusals():
         m.infer(*feats, prefix=np.zeros((2, 3), np.int32))
     with pytest.raises(ValueError, match='prefix'):
         m.infer(*feats, prefix=np.zeros((3, 3), np.int32), len_prefix=np.array([1, 4, 0]))
+    for prefix in (np.array([[1, 2, -1]] * 3), np.array([[1, 2, 10 ** 6]] * 3), np.zeros(3, np.int32), np.zeros((3, 3))):
+        with pytest.raises(ValueError, match='prefix'):
+            m.infer(*feats, prefix=prefix)
+    m.infer(*feats, prefix=np.array([[1, 2, -1]] * 3), len_prefix=np.array([2, 0, 1]))       # what lies behind the length is not read
+    with pytest.raises(ValueError, match='prefix'):
+        m.infer(*feats, len_prefix=np.array([0, 0, 0]))
+    args.sample = dict(page_size=0)
+    with pytest.raises(ValueError, match='page_size'):
+        m.infer(*feats)
+    args.sample = None
     args.decode = 'search'
     with pytest.raises(NotImplementedError, match='prefix'):
         m.infer(*feats, prefix=np.zeros((3, 3), np.int32))

@@ -118,6 +118,7 @@ def test_wrappers_refuse_what_the_c_entry_cannot_see():
            lambda: ops.paged_attention(x, kp, vp, *idx), lambda: ops.paged_attention(torch.zeros(3, 3, 8), kp, vp, *idx),
            lambda: ops.paged_attention(x, kp, vp, *idx, out=x), lambda: ops.paged_attention(x, kp, vp, *idx, scale=INF),
            lambda: ops.paged_attention(x.bfloat16(), kp, vp, *idx),
+           lambda: ops.paged_append(x.view(6, 8), x.view(6, 8), kp, vp, *idx), lambda: ops.paged_append(x, x, kp, vp, *idx, q=x.flatten()),
            lambda: ops.sample(x[0], torch.zeros(2)), lambda: ops.sample(x[0], torch.zeros(3)), lambda: ops.sample(x, torch.zeros(3)),
            lambda: ops.sample(x[0], torch.zeros(2), top_k=torch.zeros(2)), lambda: ops.sample(x[0].t(), torch.zeros(8))]
     for k, call in enumerate(bad):
