@@ -687,6 +687,53 @@ def test_replayed_graphs_and_other_streams():
     assert torch.equal(got[0], want[1][0])
 
 
+@pytest.mark.parametrize('how', ['', 'rows', 'split'])
+def test_captured_chunks_follow_the_lengths(how):
+    """one capture, replays with other lengths and contents beside eager work: two chunks' writes and attention, a workspace
+    of the caller's that both calls of the graph use in turn"""
+    t, g = torch.bfloat16, gen(67)
+    hkv, hq, dh, page = 2, 4, 64, 32
+    c = Paged(g, [150, 70, 1], [400, 70, 90], hkv, dh, page, t, fill=0.0, spare=40)
+    wide = torch.arange(3 * 16, dtype=torch.int32, device=DEV).view(3, 16)         # 512 keys each
+    c.k_pages, c.v_pages = ops.paged_cache(48, hkv, page, dh, t, DEV)
+    c.k_pages.copy_(normal(g, *c.k_pages.shape)), c.v_pages.copy_(normal(g, *c.v_pages.shape))
+    c.table = wide
+    q, table = crowded(c, normal(g, 300, hq, dh, dtype=t), how)
+    k, v = normal(g, q.shape[0], hkv, dh, dtype=t), normal(g, q.shape[0], hkv, dh, dtype=t)
+    need = ops.paged_attention_workspace_bytes(q.shape[0], *table.shape, page, hq, hkv, dh, lib.BF16)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    cu, ctx = c.cu.clone(), c.ctx_len.clone()
+    outs = [torch.full_like(q, 7.0) for _ in range(2)]
+
+    def run():
+        ops.paged_append(k, v, c.k_pages, c.v_pages, table, cu, ctx, status=c.status)
+        for causal, o in zip((True, False), outs):
+            ops.paged_attention(q, c.k_pages, c.v_pages, table, cu, ctx, causal=causal, out=o, status=c.status, workspace=ws)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for new, upto in (([150, 70, 1], [400, 70, 90]), ([1, 1, 1], [512, 1, 33]), ([0, 300, 0], [5, 301, 0]), ([100, 0, 200], [100, 64, 500])):
+        q[:300].copy_(normal(g, 300, hq, dh)), k.copy_(normal(g, *k.shape)), v.copy_(normal(g, *v.shape))
+        cu.copy_(i32([0] + list(np.cumsum(new)))), ctx.copy_(i32(upto))
+        for o in outs:
+            o.fill_(7.0)
+        run()
+        want = [o.clone() for o in outs]
+        for o in outs:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        normal(g, 100)
+        torch.cuda.synchronize()
+        assert int(c.status) == 0 and all(torch.equal(o, w) for o, w in zip(outs, want)), new
+        assert all((o[sum(new):] == 7.0).all() and not (o[:sum(new)] == 7.0).all() for o in outs)
+
+
 def test_two_streams_at_once():
     """attention and sampling on two streams at the same time have workspaces of their own"""
     g = gen(53)
