@@ -12,12 +12,12 @@
 // 2^-45 of the best have weight 0 and are never drawn.
 //
 // The kept set is {key > K} and the words with key == K up to a place, keys being the logits in an order-preserving integer
-// form.  First the words that can be kept at all are told from a bound (the top_k-th of the threads' own maxima; for top_p how
-// little the tail can weigh; min_p itself) and, up to 1024 of them, listed in index order; the rest of the work runs on that
-// list, a word a thread.  K is found by counting, not by sorting: a histogram over 1024 equal steps of (max - l) / T in
-// [0, 32) - all that can have weight - finds the step where the count passes top_k or the sum passes top_p, and the words of
-// that one step, a dozen as a rule, are ranked among each other.  (Without the list every pass ran over the row: the 256 rows
-// below took 86 us.)
+// form.  First the words that can be kept at all are told from a bound (the top_k-th of the threads' own maxima; for top_p the
+// step in which the row's sum passes it; min_p itself) and, up to 1024 of them, listed in index order; the rest of the work
+// runs on that list, a word a thread.  K is found by counting, not by sorting: a histogram over 1024 equal steps of
+// (max - l) / T in [0, 32) - all that can have weight - finds the step where the count passes top_k or the sum passes top_p,
+// and the words of that one step, a dozen as a rule, are ranked among each other.  (Without the list every pass ran over the
+// row: the 256 rows below took 86 us.)
 //
 // One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
 // the chain of passes and barriers: one row of 10000 words with top_p takes 17 us, 256 rows of 32003 words with every filter,
@@ -117,7 +117,7 @@ template <typename T, int NT> struct SampleShared {
   uint32_t hc[SAMPLE_BINS];
   int list_at[SAMPLE_LIST];
   uint32_t wa[16], wb[16], bin_c, found_key, count;
-  float wf[16], wr[16];      // maxima, sums of roots of the waves
+  float wf[16];              // maxima of the waves
   int bin, found_at, place;
   T list[SAMPLE_LIST];
 };
@@ -182,6 +182,12 @@ struct SampleRule {
   }
 };
 
+// what the sum of the words kept by top_p has to reach
+__device__ __forceinline__ u64 sample_need(float top_p, u64 total) {
+  const u64 need = (u64)ceil((double)top_p * (double)total);
+  return need < 1 ? 1 : need;
+}
+
 struct SampleLimit {         // words with key > K, and with key == K up to place `cut`
   uint32_t K;
   int cut;
@@ -223,15 +229,13 @@ template <typename T, int NT> __device__ __forceinline__ void sample_clear(Sampl
 }
 
 // The word at which the running count (by_weight: the running sum), in descending order, reaches `need`: the new limit.
-// The histogram over the words that `lim` holds, down to a step behind that word's, is in s.hc / s.hw.
+// sample_cross has found its step in the histogram over the words that `lim` holds.
 template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s,
                                                                                                                const SampleView<T, NT, CLEAN>& r,
                                                                                                    const SampleRule& rule, SampleLimit lim, u64 need,
                                                                                                    int tid) {
   constexpr int NW = NT / 64;
   const int lane = tid & 63, w = tid >> 6;
-  auto cross = [&](u64 want) { sample_cross<BY_WEIGHT>(s, want, tid); };
-  cross(need);
   const int bin = s.bin;
   if (s.bin_c <= SAMPLE_CAND) {
     // its words, ranked among each other
@@ -301,7 +305,7 @@ template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinli
       }
     });
     __syncthreads();
-    cross(need - above);
+    sample_cross<BY_WEIGHT>(s, need - above, tid);
     above += s.above;
     hi -= (uint32_t)s.bin << shift;
     const uint32_t span = (1u << shift) - 1u;
@@ -327,8 +331,9 @@ template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinli
 }
 
 // top_k, top-p and min-p over a view that holds every word that can be kept, and the draw: the place drawn in s.place, its
-// weight in s.drawn; returns the sum of the words kept.  k: 0 for none.  all: the sum over the row where top_p < 1 and no
-// top_k (the view may lack words), else not read.  Words behind step `far` are not looked at.
+// weight in s.drawn; returns the sum of the words kept.  k: 0 for none; then, where top_p < 1, `all` is the sum over the row
+// (the view may lack words) and sample_cross has found the step in which it is passed.  Words behind step `far` are not
+// looked at.
 template <typename T, int NT, bool CLEAN> __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const SampleView<T, NT, CLEAN>& r, const SampleRule& rule,
                                                                          uint32_t k, float top_p, float u, u64 all, int far, int tid) {
   constexpr int NW = NT / 64;
@@ -347,7 +352,10 @@ template <typename T, int NT, bool CLEAN> __device__ __forceinline__ u64 sample_
       }
     });
     waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
-    if (total > (u64)k) lim = sample_select<false>(s, r, rule, lim, (u64)k, tid);      // else every word with weight stays
+    if (total > (u64)k) {                                    // else every word with weight stays
+      sample_cross<false>(s, (u64)k, tid);
+      lim = sample_select<false>(s, r, rule, lim, (u64)k, tid);
+    }
   }
   if (top_p < 1.f) {
     total = all;
@@ -360,21 +368,23 @@ template <typename T, int NT, bool CLEAN> __device__ __forceinline__ u64 sample_
       __syncthreads();
       waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
     }
-    u64 need = (u64)ceil((double)top_p * (double)total);
-    if (need < 1) need = 1;
+    const u64 need = sample_need(top_p, total);
     if (need < total) {
-      sample_clear(s, tid);
-      r.each([&](float l, int place) {
-        const int b = rule.step_of(l);
-        if (b <= far && b < SAMPLE_BINS && lim.holds(logit_key(l), place)) {
-          const u64 x = rule.weight(l);
-          if (x) {
-            atomicAdd(&s.hc[b], 1u);
-            atomicAdd(&s.hw[b], x);
+      if (k) {
+        sample_clear(s, tid);
+        r.each([&](float l, int place) {
+          const int b = rule.step_of(l);
+          if (b <= far && b < SAMPLE_BINS && lim.holds(logit_key(l), place)) {
+            const u64 x = rule.weight(l);
+            if (x) {
+              atomicAdd(&s.hc[b], 1u);
+              atomicAdd(&s.hw[b], x);
+            }
           }
-        }
-      });
-      __syncthreads();
+        });
+        __syncthreads();
+        sample_cross<true>(s, need, tid);
+      }
       lim = sample_select<true>(s, r, rule, lim, need, tid);
     }
   }
@@ -486,7 +496,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
     rule.mx = mx;
     rule.exp44.init(s.roots);
     rule.inv_t = 1.0 / (double)temp;
-    rule.bin_scale = (float)(SAMPLE_BINS / SAMPLE_SPAN * rule.inv_t);
+    rule.bin_scale = (float)fmin(SAMPLE_BINS / SAMPLE_SPAN * rule.inv_t, 3e38);      // finite: wider steps do no harm
     rule.lowest = (u64)ceil((double)min_p * SAMPLE_ONE);
     const bool by_k = top_k < a.V, by_p = top_p < 1.f;
     u64 before, n, all = 0;
@@ -510,21 +520,25 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
     } else if (by_k) {
       far = SAMPLE_BINS;
     } else if (by_p) {
+      // the histogram over the row tells the step in which the sum passes top_p
       u64 mine = 0;
-      float roots = 0.f;
-      const float to_half = (float)(0.72134752 * rule.inv_t);            // exp(x / 2) as exp2
       r.each([&](float l, int) {
-        mine += rule.weight(l);
-        roots += l == mx ? 1.f : __builtin_amdgcn_exp2f((l - mx) * to_half);
+        const u64 x = rule.weight(l);
+        const int b = rule.step_of(l);
+        if (x && b < SAMPLE_BINS) {
+          atomicAdd(&s.hc[b], 1u);
+          atomicAdd(&s.hw[b], x);
+          mine += x;
+        }
       });
-      roots = wave_sum(roots);
-      if (lane == 0) s.wr[w] = roots;
       waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, all);
-      // The words behind step `far`, of weight c = e^(-far / 32) at most, weigh sum w <= sqrt(c) sum sqrt(w) together, which must
-      // not exceed what top_p leaves out (a thousandth and two steps to spare for roundings).
-      const float half = wave_sum(lane < NW ? s.wr[lane] : 0.f), rest = (float)((double)all * (1.0 - (double)top_p)) * 5.684341886e-14f;   // 2^-44
-      const float steps = 2.f * (SAMPLE_BINS / SAMPLE_SPAN) * logf(1.001f * half / rest) + 2.f;
-      far = steps < (float)SAMPLE_BINS ? (steps > 0.f ? (int)steps : 0) : SAMPLE_BINS;
+      const u64 need = sample_need(top_p, all);
+      if (need < all) {
+        sample_cross<true>(s, need, tid);
+        far = s.bin;
+      } else {
+        far = SAMPLE_BINS;
+      }
     }
     n = (u64)a.V;
     if (far < SAMPLE_BINS) {

@@ -500,6 +500,9 @@ def test_sample_odd_rows():
         uu = torch.full((x.shape[0],), u, device=DEV)
         for par in (dict(), dict(top_k=1), dict(temperature=0.0), dict(top_k=3), dict(top_p=0.5), dict(top_k=250, top_p=0.7), dict(min_p=0.5), dict(top_k=2, min_p=1.0)):
             check_rows(x, uu, ops.sample(x, uu, **par), **par)
+        tiny = 2.0 ** -133 * torch.arange(V, device=DEV)[None]      # denormal steps at the smallest normal temperature
+        for par in (dict(), dict(top_p=0.5), dict(top_k=9, top_p=0.5), dict(min_p=0.5)):
+            check_rows(tiny, uu[:1], ops.sample(tiny, uu[:1], temperature=2.0 ** -126, **par), temperature=2.0 ** -126, **par)
     # u outside [0, 1) is brought inside
     assert ops.sample(x[6:7], torch.ones(1, device=DEV))[0].item() == V - 1
     assert ops.sample(x[6:7], torch.full((1,), nan, device=DEV))[0].item() == 0
