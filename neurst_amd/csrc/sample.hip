@@ -446,14 +446,35 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   SampleView<T, NT, CACHED> r;
   r.init(CACHED ? reinterpret_cast<const T*>(row_lds) : src, a.V, tid);
   float mx = -INFINITY;
-  if constexpr (CACHED) {                                   // every lane keeps to its own words: no barrier needed
+  if constexpr (CACHED) {
+    // 16 bytes a lane (rows need not be aligned to that), four loads before the first is used; a wave reads its own words
+    constexpr int E = 16 / sizeof(T), STRIDE = 64 * E;
+    struct Words { T v[E]; };
     T* dst = reinterpret_cast<T*>(row_lds);
-#pragma unroll 8
-    for (int i = 0; i < r.steps; ++i) {
-      const int at = r.base + i * 64;
-      const float l = at < a.V ? sample_word<T>(src[at]) : -INFINITY;
-      dst[at] = (T)l;                                       // padded to whole steps
-      mx = fmaxf(mx, l);
+    const int own = r.steps * 64, w0 = w * own;
+    for (int i = lane * E; i < own; i += 4 * STRIDE) {
+      Words x[4];
+      if (a.V >= E) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = w0 + i + j * STRIDE;
+          __builtin_memcpy(&x[j], src + (i + j * STRIDE < own && at + E <= a.V ? at : 0), sizeof(Words));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = w0 + i + j * STRIDE;
+        if (i + j * STRIDE >= own) continue;
+        if (at + E > a.V)                                   // the end of the row, padded to whole steps
+          for (int e = 0; e < E; ++e) x[j].v[e] = at + e < a.V ? src[at + e] : (T)-INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float l = sample_word<T>(x[j].v[e]);
+          x[j].v[e] = (T)l;
+          mx = fmaxf(mx, l);
+        }
+        __builtin_memcpy(__builtin_assume_aligned(dst + at, 16), &x[j], 16);
+      }
     }
   } else {
     r.each([&](float l, int) { mx = fmaxf(mx, l); });
