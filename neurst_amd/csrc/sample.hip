@@ -139,8 +139,8 @@ template <typename T> __device__ __forceinline__ float sample_word(T v) {
 }
 
 // A sequence of words: place i of step and lane, in index order wave by wave, step by step, lane by lane.  CLEAN: in shared
-// memory, gone through sample_word and padded with -inf to whole steps.
-template <typename T, int NT, bool CLEAN> struct SampleView {
+// memory, gone through sample_word and padded with -inf to whole steps.  AT_ONCE: words whose chains run side by side.
+template <typename T, int NT, bool CLEAN, int AT_ONCE> struct SampleView {
   const T* p;                // [n]
   int n, base, steps;
   __device__ __forceinline__ void init(const T* p_, int n_, int tid) {
@@ -153,14 +153,14 @@ template <typename T, int NT, bool CLEAN> struct SampleView {
     if constexpr (CLEAN) return to_f32<T>(p[place]);
     return place < n ? sample_word<T>(p[place]) : -INFINITY;
   }
-  // f(word, place) for this lane's words, four read at a time; past the last step f sees -inf, which has no weight
+  // f(word, place) for this lane's words; past the last step f sees -inf, which has no weight
   template <typename F> __device__ __forceinline__ void each(F f) const {
-    for (int i = 0; i < steps; i += 4) {
-      float v[4];
+    for (int i = 0; i < steps; i += AT_ONCE) {
+      float v[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = i + j < steps ? at(base + (i + j) * 64) : -INFINITY;
+      for (int j = 0; j < AT_ONCE; ++j) v[j] = i + j < steps ? at(base + (i + j) * 64) : -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f(v[j], base + (i + j) * 64);
+      for (int j = 0; j < AT_ONCE; ++j) f(v[j], base + (i + j) * 64);
     }
   }
 };
@@ -230,10 +230,8 @@ template <typename T, int NT> __device__ __forceinline__ void sample_clear(Sampl
 
 // The word at which the running count (by_weight: the running sum), in descending order, reaches `need`: the new limit.
 // sample_cross has found its step in the histogram over the words that `lim` holds.
-template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s,
-                                                                                                               const SampleView<T, NT, CLEAN>& r,
-                                                                                                   const SampleRule& rule, SampleLimit lim, u64 need,
-                                                                                                   int tid) {
+template <bool BY_WEIGHT, typename T, int NT, typename View>
+__device__ __forceinline__ SampleLimit sample_select(SampleShared<T, NT>& s, const View& r, const SampleRule& rule, SampleLimit lim, u64 need, int tid) {
   constexpr int NW = NT / 64;
   const int lane = tid & 63, w = tid >> 6;
   const int bin = s.bin;
@@ -334,8 +332,9 @@ template <bool BY_WEIGHT, typename T, int NT, bool CLEAN> __device__ __forceinli
 // weight in s.drawn; returns the sum of the words kept.  k: 0 for none; then, where top_p < 1, `all` is the sum over the row
 // (the view may lack words) and sample_cross has found the step in which it is passed.  Words behind step `far` are not
 // looked at.
-template <typename T, int NT, bool CLEAN> __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const SampleView<T, NT, CLEAN>& r, const SampleRule& rule,
-                                                                         uint32_t k, float top_p, float u, u64 all, int far, int tid) {
+template <typename T, int NT, typename View>
+__device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const View& r, const SampleRule& rule, uint32_t k, float top_p, float u, u64 all,
+                                           int far, int tid) {
   constexpr int NW = NT / 64;
   typedef SampleShared<T, NT> S;
   const int lane = tid & 63, w = tid >> 6;
@@ -443,7 +442,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
   const int64_t row = blockIdx.x;
   extern __shared__ __attribute__((aligned(16))) char row_lds[];
   const T* src = static_cast<const T*>(a.logits) + row * a.ld;
-  SampleView<T, NT, CACHED> r;
+  SampleView<T, NT, CACHED, 4> r;
   r.init(CACHED ? reinterpret_cast<const T*>(row_lds) : src, a.V, tid);
   float mx = -INFINITY;
   if constexpr (CACHED) {
@@ -590,7 +589,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
     u64 total;
     if (n <= SAMPLE_LIST && far < SAMPLE_BINS) {
       __syncthreads();
-      SampleView<T, NT, true> few;
+      SampleView<T, NT, true, 1> few;
       few.init(s.list, (int)n, tid);
       total = sample_draw(s, few, rule, by_k ? (uint32_t)top_k : 0u, top_p, u, all, SAMPLE_BINS, tid);
       id = s.list_at[s.place];
