@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
       for (int d = 0; d < ND; ++d) acc[d] *= al;
       mx = mn;
     }
-    // the weights are rounded to the values' type for the second product (bf16: a relative 2^-9 of each, the plain form's
+    // the weights are rounded to the values' type for the second product (bf16: a relative 2^-8 of each at most, the plain form's
     // own rounding of the output is as large); their sum is taken before that, in fp32
     V p;
 #pragma unroll

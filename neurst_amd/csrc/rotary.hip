@@ -5,7 +5,9 @@
 // Bound by memory: 2 * sizeof(T) bytes an element.  A thread turns one 16-byte chunk of one head and its partner;
 // neighbouring threads hold neighbouring chunks of a head, so a wave reads whole lines.  Computing the angles once for four
 // heads a thread was slower at every size but one: the loads of the heads wait for each other (bf16, 16 heads of 96 columns:
-// 512 rows 4.3 against 3.1 us, 4000 rows 7.7 / 7.5, 8000 rows 10.6 / 11.0, 16000 rows 21.3 / 19.2 = 5.1 TB/s).
+// 512 rows 4.3 against 3.1 us, 4000 rows 7.7 / 7.5, 8000 rows 10.6 / 11.0, 16000 rows 21.3 / 19.2 = 5.1 TB/s).  Computing them
+// once a row into shared memory gains a tenth with 16 heads (16000 rows 18.7) and loses as much with nine (fp32, 4099 rows of
+// 96 columns, half of them turned: 7.9 against 7.0) or two.
 #include "rotary.h"
 
 struct RotArgs {
