@@ -113,7 +113,7 @@ struct SampleCand { u64 w; uint32_t key; int at; };
 template <typename T, int NT> struct SampleShared {
   u64 hw[SAMPLE_BINS];
   SampleCand cand[SAMPLE_CAND];
-  u64 ww[2][16], above, bin_w, drawn;
+  u64 ww[5][16], above, bin_w, drawn;
   double roots[16];
   uint32_t hc[SAMPLE_BINS];
   int list_at[SAMPLE_LIST];
@@ -123,8 +123,8 @@ template <typename T, int NT> struct SampleShared {
   T list[SAMPLE_LIST];
 };
 
-// sum over the waves before this one and over all, from each wave's own sum (the same in all its lanes); one barrier; `slot`
-// alternates so that the next call need not wait for this one's readers
+// sum over the waves before this one and over all, from each wave's own sum (the same in all its lanes); one barrier; each
+// use has a slot of its own, so that it need not wait for the last one's readers
 template <typename S, int NW> __device__ __forceinline__ void waves_sum(S& s, int slot, u64 mine, int w, int lane, u64& before, u64& all) {
   if (lane == 0) s.ww[slot][w] = mine;
   __syncthreads();
@@ -365,8 +365,7 @@ __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const View& r
         const u64 x = rule.weight(l);
         mine += lim.holds(logit_key(l), place) ? x : 0;
       });
-      __syncthreads();
-      waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
+      waves_sum<S, NW>(s, 3, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
     }
     const u64 need = sample_need(top_p, total);
     if (need < total) {
@@ -394,11 +393,19 @@ __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const View& r
   };
   u64 mine = 0;
   r.each([&](float l, int place) { mine += kept(l, place); });
-  const u64 own = readlane_u64(wave_scan_u64(mine), 63);
-  __syncthreads();                                           // the histogram and slot 0 are free
-  waves_sum<S, NW>(s, 0, own, w, lane, before, total);
+  const u64 inc = wave_scan_u64(mine), own = readlane_u64(inc, 63);
+  waves_sum<S, NW>(s, 4, own, w, lane, before, total);
   u64 thr = (u64)((double)u * (double)total);
   if (thr >= total) thr = total - 1;
+  if (r.steps == 1) {                                        // a word a lane
+    const u64 c = before + inc;
+    if (c > thr && c - mine <= thr) {
+      s.place = r.base;
+      s.drawn = mine;
+    }
+    __syncthreads();
+    return total;
+  }
   if (before <= thr && thr < before + own && lane == 0) {    // this wave's words hold the draw
     s.bin = w;
     s.above = before;
@@ -568,8 +575,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
       const float least = fminf(mx, mx - (float)(far + 2) / rule.bin_scale);
       uint32_t mine = 0;
       r.each([&](float l, int) { mine += (uint32_t)__popcll(__ballot(l >= least)); });
-      __syncthreads();
-      waves_sum<S, NW>(s, 0, (u64)mine, w, lane, before, n);
+      waves_sum<S, NW>(s, 2, (u64)mine, w, lane, before, n);
       if (n <= SAMPLE_LIST) {
         int at = (int)before;
         r.each([&](float l, int place) {
