@@ -805,8 +805,8 @@ static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t p
   // waves of a row workgroup: eight where few workgroups run (one row, 8 heads of 64 columns, 500 keys: 8 sequences 8.0 us
   // against 8.4 with four, 32 sequences 10.3 / 11.0; 64 sequences 14.9 / 13.8, 128 sequences 24.8 / 22.4)
   p.waves = p.tiles ? TILE_WAVES : wgs * p.parts <= 256 ? 8 : 4;
-  // tiles sorted by work where more workgroups are launched than run at once (three sequences of up to 4096 rows over 9000 keys,
-  // 16 heads on 4 of 128 columns: 519 us, as they come 548)
+  // tiles sorted by work (by one workgroup, so up to 2^16 of them) where more workgroups are launched than run at once (three
+  // sequences of up to 4096 rows over 9000 keys, 16 heads on 4 of 128 columns: 519 us, as they come 548)
   p.order = p.tiles && p.parts == 1 && wgs > at_once && paged_tiles(tokens, batch, group, plan_rows(p), 1) <= (1 << 16);
   return p;
 }

@@ -20,9 +20,9 @@
 // row: the 256 rows below took 86 us.)
 //
 // One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
-// the chain of passes and barriers: one row of 10000 words with top_p takes 14 us (its arg-max alone 4.1), 256 rows of 32003
-// words with every filter, a CU each, 23 us = 1.4 TB/s (the arg-max 9.5 = 3.4 TB/s); without top_k by the fp64 exponentials,
-// some 26 instructions a word: 256 rows of 32003 with top_p alone 29 us.
+// the chain of passes and barriers: one row of 10000 words with top_p takes 13 us (its arg-max alone 4.0), 256 rows of 32003
+// words with every filter, a CU each, 22 us = 1.5 TB/s (the arg-max 9.4 = 3.5 TB/s); without top_k by the fp64 exponentials,
+// some 26 instructions a word: 256 rows of 32003 with top_p alone 28 us.
 #include "common.h"
 
 struct SampleArgs {
@@ -627,8 +627,11 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
 }
 
 template <typename T> static int sample_launch(const SampleArgs& a, int64_t rows, hipStream_t s) {
-  // 1024 threads once a row gives each of them four words; 132 KB of shared memory hold the row beside the histogram
-  const int nt = a.V > 4096 ? 1024 : 256;
+  // Threads of a row, 256 / 1024 in us without filters and with top_k 50, top_p 0.95: one row of 2000 words 6.0 / 6.9 and
+  // 10.3 / 12.4, of 6000 9.5 / 8.3 and 11.9 / 12.6, of 16000 18.6 / 10.9 and 16.1 / 13.6; where rows share CUs (2048 of them)
+  // 4000 words 27 / 49 and 37 / 95, 8000 words 52 / 63 and 56 / 100, 16000 words 151 / 93 and 134 / 114.
+  // 132 KB of shared memory hold a row beside the histogram.
+  const int nt = a.V > (rows > 512 ? 8192 : 4096) ? 1024 : 256;
   const int64_t padded = cdiv64(a.V, nt) * nt, bytes = padded * (int64_t)sizeof(T);
   const bool cached = bytes <= 132 * 1024;
   static_assert(sizeof(SampleShared<T, 1024>) + 132 * 1024 <= 160 * 1024, "shared memory of a CU");

@@ -481,6 +481,14 @@ def test_sample(dtype, V, par):
     check_rows(x, u, ops.sample(x, u, **par), **par)
 
 
+def test_sample_many_rows():
+    """rows that share a CU: fewer threads a row"""
+    g = gen(71)
+    x, u = 3 * normal(g, 520, 6001), torch.rand(520, generator=g, device=DEV)
+    for par in (dict(top_p=0.9), dict(top_k=300, top_p=0.95, min_p=0.01), dict(top_k=1)):
+        check_rows(x, u, ops.sample(x, u, **par), **par)
+
+
 def test_sample_odd_rows():
     """rows with nothing to draw, infinities, NaN, the type's lowest value, signed zeros, a step between neighbours"""
     V = 501
