@@ -791,7 +791,7 @@ static AttnPlan attn_plan(int64_t tokens, int64_t batch, int64_t wide, int64_t p
   // 512 keys each (tiles, 128 rows over 4 x 8000 keys of 128 columns: 45 us, with 1024 keys 58).
   // Tiles: as many parts as all run at once, two workgroups a CU up to 128 columns, then one.  One part more than that costs a
   // second turn (3 x 700 rows x 16000 keys: 199 against 152 us; whole, 2 x 1000 x 30000: 945 against 257).
-  // Rows: a second launch joins the parts (4 us), so up to 1024 keys stay whole (4 sequences of one row, 1000 keys: 12.4 us, in
+  // Rows: a second launch joins the parts (4 to 10 us), so up to 1024 keys stay whole (4 sequences of one row, 1000 keys: 12.4 us, in
   // two parts 11.5 and a launch more; 2000 keys: 22 against 13, 16000 keys: 157 against 36); up to 4096 workgroups even out
   // ragged lengths (32 sequences, 32 heads on 8 of 128 columns, 32000 keys: 476 us, with 512 or 1024 workgroups 560).
   const int64_t at_once = dh <= 128 ? 512 : 256, least = 512;
