@@ -352,7 +352,9 @@ __device__ __forceinline__ u64 sample_draw(SampleShared<T, NT>& s, const View& r
       }
     });
     waves_sum<S, NW>(s, 0, readlane_u64(wave_scan_u64(mine), 63), w, lane, before, total);
-    if (total > (u64)k) {                                    // else every word with weight stays
+    // Else every word with weight stays.  With a bound `far` the words counted are those above it, k at least, and the words
+    // behind it are in the view all the same (too many for the list): the limit is set even where the count is k exactly.
+    if (total > (u64)k || far < SAMPLE_BINS) {
       sample_cross<false>(s, (u64)k, tid);
       lim = sample_select<false>(s, r, rule, lim, (u64)k, tid);
     }

@@ -516,6 +516,42 @@ def test_sample_odd_rows():
     assert ops.sample(x[6:7], torch.full((1,), nan, device=DEV))[0].item() == 0
 
 
+def raised_rows(V, k, t, rows=4):
+    """rows with k words 0.035 to 0.05 above a plateau of all others, every one of the k read by a lane of its own, so that
+    they fill a step of the kernel's histogram (1 / 32 at temperature 1) and the plateau the one or two behind it"""
+    nw, e = (16 if V > 4096 else 4), 128 // torch.finfo(t).bits
+    own = -(-V // (nw * 64)) * 64                              # words of a wave
+    if -(-V // (nw * 64)) * nw * 64 * torch.finfo(t).bits // 8 > 132 * 1024:
+        e = 1                                                  # rows read again from memory: a lane reads single words
+    i = torch.arange(k)
+    at = (i % nw) * own + (i // nw) * e
+    assert int(at.max()) < V and k // nw < 64
+    x = torch.zeros(rows, V)
+    x[:, at] = 0.05 - 0.015 * (torch.arange(k) % 7) / 7.0
+    x[1::2] += 1.0                                             # bf16: coarser there, all of them one value
+    return x.to(t).to(DEV)
+
+
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+@pytest.mark.parametrize('V', [3001, 5000, 32003, 70001])
+@pytest.mark.parametrize('k', [2, 8, 40, 200])
+def test_sample_top_k_ends_before_a_plateau(dtype, V, k):
+    """exactly k words lie in the steps that can hold the k-th, and more words than a list takes right behind them"""
+    x = raised_rows(V, k, TYPES[dtype])
+    for u in (0.0, 0.3, 0.6, 0.95):
+        uu = torch.full((x.shape[0],), u, device=DEV)
+        for par in (dict(), dict(min_p=0.5), dict(top_p=0.9), dict(top_p=0.5, min_p=0.97)):
+            par = dict(par, top_k=k)
+            check_rows(x, uu, ops.sample(x, uu, **par), **par)
+    R = x.shape[0]
+    preds = torch.zeros(R, 1, dtype=torch.int32, device=DEV)
+    tokens, fin, ln, left = (torch.zeros(n, dtype=torch.int32, device=DEV) for n in (R, R, R, 1))
+    scores, uu = torch.zeros(R, device=DEV), torch.linspace(0.1, 0.9, R, device=DEV)
+    ops.sample_step(x, uu, tokens, preds, fin, ln, left, scores, 0, V - 1, top_k=k, top_p=0.9)
+    check_rows(x, uu, (tokens, scores), top_k=k, top_p=0.9)
+    assert torch.equal(preds[:, 0], tokens) and int(left) == R
+
+
 def test_sample_parameters_per_row_and_strides():
     g = gen(31)
     R, V = 40, 1000
