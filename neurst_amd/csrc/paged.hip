@@ -36,13 +36,9 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) paged_appe
   const int b = paged_locate(a.ix, blockIdx.x, 1, APPEND_TILE, 2, lane, s);
   if (b < 0) return;
   if (s.bad && blockIdx.y == 0 && threadIdx.x == 0) paged_report(a.status, s.bad);
-  if (s.ctx == 0 || s.new_tokens == 0) return;
-  const int64_t tile = blockIdx.x - paged_tile_start(s.cu, 1, APPEND_TILE, 2, b);
+  int p0, p1;                                                              // positions p0 .. p1 - 1
+  if (!paged_tile_positions(s, blockIdx.x - paged_tile_start(s.cu, 1, APPEND_TILE, 2, b), APPEND_TILE, p0, p1)) return;
   const int first = s.ctx - s.new_tokens;                                  // position of the first new token
-  const int64_t lo64 = (int64_t)(first & ~(APPEND_TILE - 1)) + tile * APPEND_TILE;
-  if (lo64 >= s.ctx) return;
-  const int p0 = (int)lo64 < first ? first : (int)lo64;
-  const int p1 = lo64 + APPEND_TILE < s.ctx ? (int)lo64 + APPEND_TILE : s.ctx;   // positions p0 .. p1 - 1
   const int page = 1 << a.ix.page_log2, mask = page - 1;
   const int nt = p1 - p0, heads = a.hkv + a.hq, hgs = (heads + a.hg - 1) / a.hg;
   const int k_items = nt * hgs * a.sh.chunks;

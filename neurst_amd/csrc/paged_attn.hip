@@ -72,11 +72,7 @@ template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs
   t.b = paged_locate(a.ix, tile, a.group, ROWS, 1, lane, s);
   if (t.b < 0) return false;
   if (report && s.bad) paged_report(a.status, s.bad);
-  const int64_t own = tile - paged_tile_start(s.cu, a.group, ROWS, 1, t.b);
-  const int64_t rows = (int64_t)s.new_tokens * a.group;
-  if (own * ROWS >= rows) return false;
-  t.row_begin = (int)(own * ROWS);
-  t.n_rows = (int)(rows - own * ROWS < ROWS ? rows - own * ROWS : ROWS);
+  if (!paged_tile_rows(s, tile - paged_tile_start(s.cu, a.group, ROWS, 1, t.b), a.group, ROWS, t.row_begin, t.n_rows)) return false;
   t.row0 = s.row0;
   t.first_token = t.row_begin / a.group;
   t.last_token = (t.row_begin + t.n_rows - 1) / a.group;

@@ -4,7 +4,7 @@
 // tokens WITH them, so its row j stands at position ctx[b] - n_b + j.  Position p lives in page table[b][p >> page_log2],
 // slot p & (page - 1).
 //
-// All of it is read from device memory, where the host cannot check it, so every use goes through the two functions below:
+// All of it is read from device memory, where the host cannot check it, so every use goes through the functions below:
 // lengths that do not fit leave the sequence out, a page id outside the pool leaves its keys out, and both raise a bit of
 // the caller's status word.  Nothing is read or written out of range whatever the four arrays hold.
 #pragma once
@@ -76,7 +76,8 @@ static inline int64_t paged_tiles(int64_t tokens, int64_t batch, int64_t mult, i
 
 // The sequence a tile belongs to: the last b with tile_start(b) <= tile, -1 for none.  count(lo, step, width) says how many of
 // the at most 64 candidates lo, lo + step, .. below lo + width start at or before the tile.  cu that does not grow gives some
-// sequence or none, never an index out of range.
+// sequence or none, never an index out of range; that sequence may begin behind the tile, so what the tile is of it goes
+// through one of the two functions below.
 template <typename Count> NEURST_HD int paged_search(int batch, Count count) {
   int lo = 0, width = batch;
   for (;;) {
@@ -88,4 +89,24 @@ template <typename Count> NEURST_HD int paged_search(int batch, Count count) {
     width = lo + width - last < step ? lo + width - last : step;
     lo = last;
   }
+}
+
+// Rows begin .. begin + count - 1 of a sequence's new_tokens * mult that its tile `own` of `per` rows has; false: none
+NEURST_HD bool paged_tile_rows(const PagedSeq& s, int64_t own, int64_t mult, int per, int& begin, int& count) {
+  const int64_t rows = (int64_t)s.new_tokens * mult;
+  if (own < 0 || own * per >= rows) return false;
+  begin = (int)(own * per);
+  count = (int)(rows - own * per < per ? rows - own * per : per);
+  return true;
+}
+// Positions p0 .. p1 - 1 of a sequence's new tokens in its tile `own` of `per` (a power of two) positions aligned in the
+// cache; false: none
+NEURST_HD bool paged_tile_positions(const PagedSeq& s, int64_t own, int per, int& p0, int& p1) {
+  if (own < 0 || s.ctx == 0 || s.new_tokens == 0) return false;
+  const int first = s.ctx - s.new_tokens;
+  const int64_t lo = (int64_t)(first & ~(per - 1)) + own * per;
+  if (lo >= s.ctx) return false;
+  p0 = lo < first ? first : (int)lo;
+  p1 = lo + per < s.ctx ? (int)(lo + per) : s.ctx;
+  return true;
 }

@@ -25,6 +25,15 @@ def test_index_arithmetic_of_the_paged_cache(tmp_path):
     assert r.returncode == 0 and r.stdout.strip() == 'ok', r.stdout + r.stderr
 
 
+def test_rows_and_positions_of_the_tiles_stay_with_their_sequences(tmp_path):
+    """starts that do not grow, rows past the tensors: what a tile reads and writes lies inside its sequence's rows"""
+    exe = str(tmp_path / 'check')
+    src = os.path.join(ROOT, 'tests', 'native', 'check_paged_tiles.cpp')
+    subprocess.run(['g++', '-O2', '-std=c++17', '-fsanitize=address,undefined', src, '-o', exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == 'ok', r.stdout + r.stderr
+
+
 def _call(name, good, **change):
     args = dict(good, **change)
     return getattr(lib.load(), name)(*args.values())
