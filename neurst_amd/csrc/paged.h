@@ -28,6 +28,14 @@ __device__ __forceinline__ void paged_report(int32_t* status, int bits) {
   if (status && bits) atomicOr(status, bits);
 }
 
+// The last workgroup of a launch looks over every sequence's lengths and does nothing else: tiles alone would not do, since
+// none leads to a sequence behind a start that is out of range.  It runs beside the others and costs a call nothing.
+__device__ __forceinline__ void paged_look_over(const PagedIndex& x, int32_t* status) {
+  int bad = 0;
+  for (int b = threadIdx.x; b < x.batch; b += blockDim.x) bad |= paged_seq(x, b).bad;
+  paged_report(status, bad);
+}
+
 #define PAGED_CHECK_INDEX(name)                                                                                            \
   NEURST_CHECK_ARG(page_table && cu_new && ctx_len, name ": null index pointer");                                           \
   NEURST_CHECK_ARG(tokens >= 0 && tokens <= INT32_MAX && batch >= 0 && batch <= (1 << 20), name ": bad token or sequence count"); \

@@ -31,11 +31,14 @@ constexpr int APPEND_TILE = 64;
 
 template <typename T, int VEC> __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
   constexpr int E = 16 / sizeof(T);          // slots of a value item, and its columns
+  if (blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.y == 0) paged_look_over(a.ix, a.status);
+    return;
+  }
   const int lane = threadIdx.x & 63;
   PagedSeq s;
   const int b = paged_locate(a.ix, blockIdx.x, 1, APPEND_TILE, 2, lane, s);
   if (b < 0) return;
-  if (s.bad && blockIdx.y == 0 && threadIdx.x == 0) paged_report(a.status, s.bad);
   int p0, p1;                                                              // positions p0 .. p1 - 1
   if (!paged_tile_positions(s, blockIdx.x - paged_tile_start(s.cu, 1, APPEND_TILE, 2, b), APPEND_TILE, p0, p1)) return;
   const int first = s.ctx - s.new_tokens;                                  // position of the first new token
@@ -123,7 +126,7 @@ template <typename T> static int append_launch(AppendArgs a, int64_t pairs, int 
   const int64_t items = per * a.sh.chunks * cdiv64(heads, a.hg) + cdiv64(per, 16 / es) * (a.dh / (16 / es)) * a.hkv;
   int64_t gy = cdiv64(items, 256);      // one item a thread (37 sequences of up to 700: 30.5 us; two items 31.9, four 33.6)
   if (gy > 64) gy = 64;
-  const dim3 grid((unsigned)tiles, (unsigned)gy);
+  const dim3 grid((unsigned)tiles + 1, (unsigned)gy);      // the last one: paged_look_over
   switch (vec) {
     case 8: if constexpr (sizeof(T) == 2) paged_append_kernel<T, 8><<<grid, 256, 0, s>>>(a); break;
     case 4: paged_append_kernel<T, 4><<<grid, 256, 0, s>>>(a); break;

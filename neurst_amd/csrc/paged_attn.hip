@@ -67,11 +67,10 @@ struct RowTile {
   int shift;                                                  // position of token 0
   int row_begin;                                              // first of the tile's rows within the sequence
 };
-template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs& a, int64_t tile, int lane, RowTile& t, bool report) {
+template <int ROWS> __device__ __forceinline__ bool row_tile(const PagedAttnArgs& a, int64_t tile, int lane, RowTile& t) {
   PagedSeq s;
   t.b = paged_locate(a.ix, tile, a.group, ROWS, 1, lane, s);
   if (t.b < 0) return false;
-  if (report && s.bad) paged_report(a.status, s.bad);
   if (!paged_tile_rows(s, tile - paged_tile_start(s.cu, a.group, ROWS, 1, t.b), a.group, ROWS, t.row_begin, t.n_rows)) return false;
   t.row0 = s.row0;
   t.first_token = t.row_begin / a.group;
@@ -101,8 +100,12 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   // heads first: with a multiple of eight of them, or a divisor, an XCD sees few heads' keys through its L2
   const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (z == 0) paged_look_over(a.ix, a.status);
+    return;
+  }
   RowTile t;
-  if (!row_tile<16>(a, blockIdx.x / (unsigned)a.hkv, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  if (!row_tile<16>(a, blockIdx.x / (unsigned)a.hkv, lane, t)) return;
   const int dh = EXACT ? DH : a.dh;
   const int page = 1 << a.ix.page_log2, pmask = page - 1;
   // this lane's query: row m of the tile
@@ -366,10 +369,14 @@ __global__ void __launch_bounds__(TILE_WAVES * 64, DH <= 128 ? 2 : 1) paged_attn
   extern __shared__ __attribute__((aligned(1024))) char smem[];                 // keys [2], values [2], what `clean` notes
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
   const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (z == 0) paged_look_over(a.ix, a.status);
+    return;
+  }
   RowTile t;
   int64_t tile = blockIdx.x / (unsigned)a.hkv;
   if (a.order) tile = a.order[tile];
-  if (!row_tile<ROWS>(a, tile, lane, t, tid == 0 && kvh == 0 && z == 0)) return;
+  if (!row_tile<ROWS>(a, tile, lane, t)) return;
   const int dh = EXACT ? DH : a.dh;
   const int page = 1 << a.ix.page_log2, pmask = page - 1;
   const int row = 32 * w + m;
@@ -840,7 +847,7 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   }
   const int per = plan_rows(plan);
   a.tiles = paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1);
-  const dim3 grid((unsigned)(a.tiles * a.hkv), (unsigned)a.parts);
+  const dim3 grid((unsigned)(a.tiles * a.hkv) + 1, (unsigned)a.parts);      // the last one: paged_look_over
   if (plan.order) {
     a.order = static_cast<int32_t*>(ws);
     paged_attn_order<<<1, 1024, 0, s>>>(a, per);

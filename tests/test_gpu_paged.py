@@ -404,6 +404,34 @@ def test_bad_pages_and_lengths_are_left_out(n, how):
         assert same(c.k_pages, kp) and same(c.v_pages, vp)
 
 
+@pytest.mark.parametrize('n,how', [(1, ''), (40, ''), (40, 'rows'), (40, 'split')])
+def test_lengths_that_no_tile_leads_to_are_reported(n, how):
+    """all rows past the tensors: no workgroup finds a sequence, the status tells all the same; correct lengths leave it zero"""
+    t, g = torch.bfloat16, gen(73)
+    hkv, dh, page = 2, 64, 16
+    c = Paged(g, [n, n, n], [n + 40, n + 40, n + 40], hkv, dh, page, t).put()
+    q, c.table = crowded(c, normal(g, 3 * n, hkv, dh, dtype=t), how)
+    tokens = q.shape[0]
+    k = normal(g, 3 * n, hkv, dh, dtype=t)
+    bits = lambda x: x.view(torch.int16)
+    kp, vp = c.k_pages.clone(), c.v_pages.clone()
+    for cu in ([tokens + 1] * 4, [2 ** 31 - 1] * 4, [tokens + 5, tokens + 6, tokens + 7, tokens + 9]):
+        for causal in (True, False):
+            c.status.zero_()
+            out = torch.full_like(q, 7.0)
+            ops.paged_attention(q, kp, vp, c.table, i32(cu), c.ctx_len, causal=causal, out=out, status=c.status)
+            assert int(c.status) == 2 and (out == 7.0).all(), cu
+        c.status.zero_()
+        ops.paged_append(k, k, kp, vp, c.table, i32(cu), c.ctx_len, status=c.status)
+        assert int(c.status) == 2 and torch.equal(bits(kp), bits(c.k_pages)) and torch.equal(bits(vp), bits(c.v_pages)), cu
+    c.status.zero_()
+    ops.paged_attention(q, kp, vp, *c.index(), status=c.status)
+    ops.paged_append(k, k, kp, vp, *c.index(), status=c.status)
+    ops.paged_check(c.status)
+    with pytest.raises(lib.NeurstLibError, match='lengths'):
+        ops.paged_check(c.status.fill_(2))
+
+
 def test_offsets_beyond_32_bits():
     """the pool holds more than 2^32 elements; the sequence's pages lie at its end"""
     t, g = torch.bfloat16, gen(29)
