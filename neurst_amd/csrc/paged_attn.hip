@@ -739,14 +739,16 @@ __global__ void __launch_bounds__(1024) paged_attn_order(PagedAttnArgs a, int ro
   for (int64_t i = tid; i < a.tiles; i += 1024) a.order[atomicAdd(&first[class_of(i)], 1u)] = (int32_t)i;
 }
 
-// joins the parts: one wave a row (token x head)
-template <typename T>
+// Joins the parts: one wave a row (token x head).  The rows are found by the tiles that wrote the parts, so that rows no
+// sequence owns - behind the last one, or of lengths that were refused - are left as they were, like those of whole keys.
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw, int64_t rows) {
   const int lane = threadIdx.x & 63, heads = a.hkv * a.group;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int64_t token = row / heads;
-  if (token < a.ix.cu[0] || token >= a.ix.cu[a.ix.batch]) return;      // rows of no sequence stay as they were
+  const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), own = blockIdx.y * 4 + (threadIdx.x >> 6);
+  RowTile t;
+  if (!row_tile<ROWS>(a, blockIdx.x / (unsigned)a.hkv, lane, t) || own >= t.n_rows) return;
+  const int r = t.row_begin + own;
+  const int64_t token = t.row0 + r / a.group, row = token * heads + kvh * a.group + r % a.group;
   // lane z holds part z's maximum and sum (at most 64 parts), and what its partial result counts
   float pm = -INFINITY, pl = 0.f;
   if (lane < a.parts) {
@@ -882,7 +884,11 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   }
   NEURST_CHECK_LAUNCH("paged_attention");
   if (a.parts > 1) {
-    paged_attn_join<T><<<(unsigned)cdiv64(rows, 4), 256, 0, s>>>(a, pd, rows);
+    const dim3 joins((unsigned)(a.tiles * a.hkv), (unsigned)(per / 4));
+    if constexpr (sizeof(T) == 2) {
+      if (plan.tiles) paged_attn_join<T, 32 * TILE_WAVES><<<joins, 256, 0, s>>>(a, pd, rows);
+    }
+    if (!plan.tiles) paged_attn_join<T, 16><<<joins, 256, 0, s>>>(a, pd, rows);
     NEURST_CHECK_LAUNCH("paged_attention join");
   }
   return NEURST_OK;

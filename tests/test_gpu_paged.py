@@ -432,6 +432,43 @@ def test_lengths_that_no_tile_leads_to_are_reported(n, how):
         ops.paged_check(c.status.fill_(2))
 
 
+@pytest.mark.parametrize('dtype,n,how', [('bf16', 1, ''), ('bf16', 40, ''), ('fp32', 40, ''), ('bf16', 40, 'rows'), ('bf16', 40, 'split'),
+                                         ('bf16', 1, 'long'), ('bf16', 40, 'long'), ('fp32', 1, 'long'), ('fp32', 40, 'long')])
+def test_rows_of_refused_sequences_stay_as_they_are(dtype, n, how):
+    """cu_new that does not fit, with whole keys and with parts of them, whatever the workspace holds ('long': the kernel for few
+    rows over a table of 8192 keys)"""
+    t, g = TYPES[dtype], gen(79)
+    hkv, dh, page = 2, 64, 16
+    c = Paged(g, [n, n, n], [n + 40, n + 40, n + 40], hkv, dh, page, t).put()
+    q = normal(g, 3 * n, hkv, dh, dtype=t)
+    if how == 'long':
+        c.table = torch.cat([c.table, torch.full((3, 8192 // page - c.table.shape[1]), -1, dtype=torch.int32, device=DEV)], 1)
+    else:
+        q, c.table = crowded(c, q, how)
+    tokens, far = q.shape[0], 2 ** 30
+    need = ops.paged_attention_workspace_bytes(tokens, 3, c.table.shape[1], page, hkv, hkv, dh, ops.dt_of(q))
+    parts = need >= 2 * tokens * hkv * dh * 4
+    assert parts == (how in ('split', 'long'))
+    ws = torch.empty(max(need, 16) // 4, device=DEV)
+
+    def attend_with(cu):
+        ws.fill_(3.0)
+        c.status.zero_()
+        out = torch.full_like(q, 7.0)
+        ops.paged_attention(q, c.k_pages, c.v_pages, c.table, i32(cu), c.ctx_len, out=out, status=c.status, workspace=ws)
+        return out
+
+    good = attend_with([0, n, 2 * n, 3 * n])
+    assert int(c.status) == 0 and (good[3 * n:] == 7.0).all()
+    for cu, kept in (([0, n, far, 3 * n], [(0, n)]), ([-5, n, 2 * n, 3 * n], [(n, 3 * n)]), ([0, n, 2 * n, far], [(0, 2 * n)]),
+                     ([0, n, tokens + 1, 3 * n], [(0, n)])):
+        got = attend_with(cu)
+        want = torch.full_like(q, 7.0)
+        for a, b in kept:
+            want[a:b] = good[a:b]
+        assert int(c.status) == 2 and torch.equal(got, want), cu
+
+
 def test_offsets_beyond_32_bits():
     """the pool holds more than 2^32 elements; the sequence's pages lie at its end"""
     t, g = torch.bfloat16, gen(29)
