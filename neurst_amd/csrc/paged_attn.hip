@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
           const f32x4 x = *reinterpret_cast<const f32x4*>(&red[i][orow][c]);
-          if (f[i] != 0.f) v += x * f[i];
+          v += x * f[i];
         }
         if (a.parts == 1) {
           T* op = static_cast<T*>(a.o) + grow * a.ldo + (int64_t)hd * dh + dim;
@@ -756,12 +756,14 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw,
     pm = a.ws_ml[at];
     pl = a.ws_ml[at + 1];
   }
-  const float M = wave_max(pm), f = fast_exp2(pm - safe_max(M)), L = wave_sum(f == 0.f ? 0.f : f * pl);
+  const float M = wave_max(pm), f = fast_exp2(pm - safe_max(M)), L = wave_sum(f * pl);
   f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
   const int dim = lane * 4;
   for (int z = 0; z < a.parts; ++z) {
     const float fz = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), z));
-    if (fz != 0.f && dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + (z * rows + row) * ldw + dim) * fz;
+    // a sum of 0: the row sees nothing there and no partial result was written; one that counts for nothing (fz 0) is added all
+    // the same, as a NaN of it has to reach the result
+    if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, pl), z) != 0 && dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + (z * rows + row) * ldw + dim) * fz;
   }
   if (dim >= a.dh) return;
   const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);

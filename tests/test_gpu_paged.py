@@ -346,6 +346,56 @@ def test_masked_values_that_are_not_finite(dtype, how, n, dh):
     assert torch.isnan(got[cut + 3:]).all()
 
 
+@pytest.mark.parametrize('dtype,n,wide,how', [('bf16', 1, 8192, ''), ('fp32', 1, 8192, ''), ('bf16', 20, 8192, ''), ('bf16', 40, 4096, 'split'),
+                                              ('bf16', 40, 1024, ''), ('fp32', 40, 1024, '')])
+def test_what_is_not_finite_and_seen_reaches_the_result(dtype, n, wide, how):
+    """a query, a key or a value that a row sees is NaN or infinite, wherever the keys are split and however little the value
+    counts: the row is not finite, and others stay as they are"""
+    t, g = TYPES[dtype], gen(83)
+    hkv, dh, page, ctx = 2, 64, 16, 3000 if wide > 3000 else 900
+    c = Paged(g, [n], [ctx], hkv, dh, page, t, fill=0.0)
+    c.k_pages.copy_(normal(g, *c.k_pages.shape)), c.v_pages.copy_(normal(g, *c.v_pages.shape))
+    c.table = torch.cat([c.table, torch.full((1, wide // page - c.table.shape[1]), -1, dtype=torch.int32, device=DEV)], 1)
+    q = normal(g, n, hkv, dh, dtype=t)
+    q[:, :, 0] = 1.0
+    far = 700                                                  # one key that counts for nothing, in fp32 exactly
+    c.k_pages[c.rows[0][far // page], :, far % page] = 0.0
+    c.k_pages[c.rows[0][far // page], :, far % page, 0] = -2.0 ** 14
+    many, c.table = crowded(c, q, how)
+    need = ops.paged_attention_workspace_bytes(many.shape[0], *c.table.shape, page, hkv, hkv, dh, ops.dt_of(q))
+    assert (need >= 2 * many.shape[0] * hkv * dh * 4) == (wide > 1024)
+    run = lambda: ops.paged_attention(many, c.k_pages, c.v_pages, *c.index())[:n]
+    good = run()
+    assert torch.isfinite(good).all()
+    bad = many.clone()
+    bad[0, 1, 5] = float('nan')
+    got = ops.paged_attention(bad, c.k_pages, c.v_pages, *c.index())[:n]
+    assert torch.isnan(got[0, 1]).all() and torch.equal(got[0, 0], good[0, 0]) and torch.equal(got[1:], good[1:])
+    for at in (3, 600, far, ctx - n):
+        pg, slot = c.rows[0][at // page], at % page
+        for value in (float('nan'), float('inf'), -float('inf')):
+            if at != far and value != value:
+                kept = c.k_pages[pg, 0, slot].clone()
+                c.k_pages[pg, 0, slot, 7] = value
+                got = run()
+                assert torch.isnan(got[:, 0]).all() and torch.equal(got[:, 1], good[:, 1]), ('key', at)
+                c.k_pages[pg, 0, slot] = kept
+            kept = c.v_pages[pg, 1, 9, slot].clone()
+            c.v_pages[pg, 1, 9, slot] = value
+            got = run()
+            assert not torch.isfinite(got[:, 1, 9]).any(), ('value', at, value)
+            rest = torch.arange(dh, device=DEV) != 9
+            assert torch.equal(got[:, 0], good[:, 0]) and torch.equal(got[:, 1, rest], good[:, 1, rest]), ('value', at, value)
+            c.v_pages[pg, 1, 9, slot] = kept
+    # a part whose only keys are NaN
+    pages = c.rows[0][512 // page:1024 // page if wide > 1024 else 800 // page]
+    kept = c.k_pages[pages].clone()
+    c.k_pages[pages] = float('nan')
+    assert torch.isnan(run()).all()
+    c.k_pages[pages] = kept
+    assert torch.equal(run(), good)
+
+
 def test_pages_shared_by_sequences():
     """hypotheses of one utterance against the same pages, and one key page for every position"""
     t, g = torch.bfloat16, gen(19)
