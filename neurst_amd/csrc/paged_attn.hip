@@ -100,8 +100,8 @@ __global__ void __launch_bounds__(NW * 64, DH <= 64 ? 4 : DH <= 96 ? 3 : DH <= 1
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   // heads first: with a multiple of eight of them, or a divisor, an XCD sees few heads' keys through its L2
   const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
-  if (blockIdx.x == gridDim.x - 1) {
-    if (z == 0) paged_look_over(a.ix, a.status);
+  if (blockIdx.x / (unsigned)a.hkv == a.tiles) {
+    if (kvh == 0 && z == 0) paged_look_over(a.ix, a.status);
     return;
   }
   RowTile t;
@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(TILE_WAVES * 64, DH <= 128 ? 2 : 1) paged_attn
   extern __shared__ __attribute__((aligned(1024))) char smem[];                 // keys [2], values [2], what `clean` notes
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 31, h = lane >> 5;
   const int kvh = (int)(blockIdx.x % (unsigned)a.hkv), z = blockIdx.y;
-  if (blockIdx.x == gridDim.x - 1) {
-    if (z == 0) paged_look_over(a.ix, a.status);
+  if (blockIdx.x / (unsigned)a.hkv == a.tiles) {
+    if (kvh == 0 && z == 0) paged_look_over(a.ix, a.status);
     return;
   }
   RowTile t;
@@ -748,7 +748,8 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw,
   RowTile t;
   if (!row_tile<ROWS>(a, blockIdx.x / (unsigned)a.hkv, lane, t) || own >= t.n_rows) return;
   const int r = t.row_begin + own;
-  const int64_t token = t.row0 + r / a.group, row = token * heads + kvh * a.group + r % a.group;
+  const int head = kvh * a.group + r % a.group;
+  const int64_t token = t.row0 + r / a.group, row = token * heads + head;
   // lane z holds part z's maximum and sum (at most 64 parts), and what its partial result counts
   float pm = -INFINITY, pl = 0.f;
   if (lane < a.parts) {
@@ -763,14 +764,15 @@ __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw,
     const float fz = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), z));
     // a sum of 0: the row sees nothing there and no partial result was written; one that counts for nothing (fz 0) is added all
     // the same, as a NaN of it has to reach the result
-    if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, pl), z) != 0 && dim < a.dh) v += *reinterpret_cast<const f32x4*>(a.ws_o + (z * rows + row) * ldw + dim) * fz;
+    if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, pl), z) != 0 && dim < a.dh)
+      v += *reinterpret_cast<const f32x4*>(a.ws_o + (z * rows + row) * ldw + dim) * fz;
   }
   if (dim >= a.dh) return;
   const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
   T out[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = from_f32<T>(v[j] * inv);
-  T* op = static_cast<T*>(a.o) + token * a.ldo + (row % heads) * a.dh + dim;
+  T* op = static_cast<T*>(a.o) + token * a.ldo + (int64_t)head * a.dh + dim;
   __builtin_memcpy(__builtin_assume_aligned(op, 4 * sizeof(T)), out, sizeof(out));
 }
 
@@ -851,7 +853,9 @@ template <typename T> static int attn_launch(PagedAttnArgs a, AttnPlan plan, voi
   }
   const int per = plan_rows(plan);
   a.tiles = paged_tiles(a.ix.tokens, a.ix.batch, a.group, per, 1);
-  const dim3 grid((unsigned)(a.tiles * a.hkv) + 1, (unsigned)a.parts);      // the last one: paged_look_over
+  // behind the tiles one more workgroup for paged_look_over: a whole tile's, so that a head stays with its XCD in every part
+  // (three sequences of up to 700 rows over 16000 keys in five parts: 98 us, with a single one 104)
+  const dim3 grid((unsigned)((a.tiles + 1) * a.hkv), (unsigned)a.parts);
   if (plan.order) {
     a.order = static_cast<int32_t*>(ws);
     paged_attn_order<<<1, 1024, 0, s>>>(a, per);
