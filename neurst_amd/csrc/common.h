@@ -27,6 +27,18 @@ void neurst_set_error(const char* fmt, ...);
     }                                                \
   } while (0)
 
+// Whether two tensors of `rows` rows, `width` bytes at every `stride`, share memory.  Rows of equal strides may lie between
+// each other (slices of one packed buffer); of unequal ones everything from the first to the last byte counts.
+struct Rows { const void* p; int64_t width, stride, rows; };
+static inline bool rows_meet(const Rows& a, const Rows& b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  if (pa + (uintptr_t)((a.rows - 1) * a.stride + a.width) <= pb || pb + (uintptr_t)((b.rows - 1) * b.stride + b.width) <= pa) return false;
+  if (a.stride != b.stride || a.rows == 1 || b.rows == 1) return true;
+  const int64_t d = (int64_t)(pb > pa ? (pb - pa) % (uintptr_t)a.stride : ((uintptr_t)a.stride - (pa - pb) % (uintptr_t)a.stride) % (uintptr_t)a.stride);
+  return !(d >= a.width && d + b.width <= a.stride);
+}
+
 #define NEURST_CHECK_LAUNCH(name)                                              \
   do {                                                                         \
     hipError_t e_ = hipGetLastError();                                         \

@@ -157,6 +157,13 @@ extern "C" int neurst_paged_append(const void* k, const void* v, const void* q, 
                           (uintptr_t)(ldk * es) | (uintptr_t)(ldv * es) | (q ? (uintptr_t)(ldq * es) | (uintptr_t)(ldqo * es) : 0);
   NEURST_CHECK_ARG(align % 16 == 0, "paged_append: pointers and row strides must be 16-byte aligned");
   if (tokens == 0 || batch == 0) return NEURST_OK;
+  const Rows rk = {k, kv_heads * dh * es, ldk * es, tokens}, rv = {v, kv_heads * dh * es, ldv * es, tokens}, rq = {q, q_heads * dh * es, ldq * es, tokens},
+             ro = {q_out, q_heads * dh * es, ldqo * es, tokens}, kp = {k_pages, n_pages * page_size * kv_heads * dh * es, 0, 1}, vp = {v_pages, kp.width, 0, 1};
+  NEURST_CHECK_ARG(!rows_meet(ro, rk) && !rows_meet(ro, rv) && (q == q_out || !rows_meet(ro, rq)),
+                   "paged_append: q_out must be q itself or apart from it, and apart from k and v");
+  NEURST_CHECK_ARG(!rows_meet(kp, vp) && !rows_meet(kp, rk) && !rows_meet(kp, rv) && !rows_meet(kp, rq) && !rows_meet(kp, ro) && !rows_meet(vp, rk) &&
+                       !rows_meet(vp, rv) && !rows_meet(vp, rq) && !rows_meet(vp, ro),
+                   "paged_append: k_pages and v_pages must be apart from each other and from k, v, q and q_out");
   AppendArgs a;
   a.ix = paged_index(page_table, cu_new, ctx_len, tokens, batch, wide, ld_table, page_size, n_pages, true);
   a.k = k; a.v = v; a.q = q; a.k_pages = k_pages; a.v_pages = v_pages; a.q_out = q_out; a.freq = freq; a.status = status;

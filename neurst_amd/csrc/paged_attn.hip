@@ -930,5 +930,11 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   const int64_t need = neurst_paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_heads, dh, dtype);
   NEURST_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                    "paged_attention: the workspace must hold neurst_paged_attention_workspace_bytes() bytes, 16-byte aligned");
+  const int64_t pool = n_pages * page_size * kv_heads * dh * es;
+  const Rows ro = {o, q_heads * dh * es, ldo * es, tokens}, rq = {q, q_heads * dh * es, ldq * es, tokens}, kp = {k_pages, pool, 0, 1}, vp = {v_pages, pool, 0, 1},
+             ws = {workspace, need, 0, 1};
+  NEURST_CHECK_ARG(!rows_meet(ro, rq) && !rows_meet(ro, kp) && !rows_meet(ro, vp), "paged_attention: o must be apart from q and the pages");
+  NEURST_CHECK_ARG(!rows_meet(ws, ro) && !rows_meet(ws, rq) && !rows_meet(ws, kp) && !rows_meet(ws, vp),
+                   "paged_attention: the workspace must be apart from q, o and the pages");
   return dtype == NEURST_BF16 ? attn_launch<bf16_t>(a, plan, workspace, as_stream(stream)) : attn_launch<float>(a, plan, workspace, as_stream(stream));
 }

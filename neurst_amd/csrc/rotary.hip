@@ -84,6 +84,8 @@ extern "C" int neurst_rotary(const void* x, void* y, const double* freq, const i
     NEURST_CHECK_ARG((((uintptr_t)x | (uintptr_t)y | (uintptr_t)(ldx * es) | (uintptr_t)(ldy * es) | (uintptr_t)(dh * es)) % (2 * es)) == 0,
                      "rotary: interleaved pairs must be aligned to two elements");
   if (rows == 0) return NEURST_OK;
+  NEURST_CHECK_ARG(x == y || !rows_meet(Rows{x, heads * dh * es, ldx * es, rows}, Rows{y, heads * dh * es, ldy * es, rows}),
+                   "rotary: y must be x or apart from it");
   RotArgs a;
   a.x = x; a.y = y; a.freq = freq; a.pos = positions;
   a.ldx = ldx; a.ldy = ldy; a.period = (uint32_t)period; a.heads = (int)heads; a.pos0 = (int)pos0;

@@ -198,6 +198,31 @@ def test_paged_append(dtype, lengths, hkv, hq, dh, page, rot, layout):
     assert torch.equal(bits(c.k_pages)[~seen_k], bits(before_k)[~seen_k]) and torch.equal(bits(c.v_pages)[~seen_v], bits(before_v)[~seen_v])
 
 
+def test_paged_append_in_place_of_a_packed_projection():
+    """queries turned where they lie between the keys and values; queries that are the keys are refused"""
+    t, g = torch.bfloat16, gen(89)
+    c = Paged(g, [70, 5], [70, 40], 2, 64, 16, t)
+    packed = normal(g, 75, 6 * 64, dtype=t)
+    freq = ops.rotary_frequencies(64, device=DEV)[0]
+    parts = lambda x: x.unflatten(1, (6, 64)).split([2, 2, 2], 1)
+    q, k, v = parts(packed.clone())
+    want = ops.paged_append(k, v, c.k_pages, c.v_pages, *c.index(), q=q, freq=freq)
+    keys, values = c.k_pages.clone(), c.v_pages.clone()
+    q, k, v = parts(packed)
+    kept = k.clone(), v.clone()
+    assert ops.paged_append(k, v, c.k_pages, c.v_pages, *c.index(), q=q, q_out=q, freq=freq) is q
+    bits = lambda x: x.contiguous().view(torch.int16)
+    assert torch.equal(q, want) and torch.equal(bits(keys), bits(c.k_pages)) and torch.equal(bits(values), bits(c.v_pages))
+    assert torch.equal(k, kept[0]) and torch.equal(v, kept[1])
+    for other in (k, v):
+        with pytest.raises((ValueError, lib.NeurstLibError), match='apart'):
+            ops.paged_append(k, v, c.k_pages, c.v_pages, *c.index(), q=other, q_out=other, freq=freq)
+    square = torch.zeros(4, 2, 64, 64, dtype=t, device=DEV)      # page_size 64, dh 64: both pools have one shape
+    with pytest.raises((ValueError, lib.NeurstLibError), match='apart'):
+        ops.paged_append(k, v, square, square, i32([[0, 1], [2, 3]]), c.cu, c.ctx_len)
+    assert torch.equal(k, kept[0]) and not square.any()
+
+
 def attend(c, q, causal=True, scale=None):
     """fp64 result and the bound of the docstring"""
     dh, t = q.shape[2], q.dtype

@@ -83,6 +83,25 @@ def test_paged_attention_refuses(change):
     assert b'paged_attention' in lib.load().neurst_last_error()
 
 
+def test_memory_that_is_written_must_be_apart():
+    """in place and interleaved slices of one packed projection are fine (the GPU tests make those calls); what another part of the
+    call reads is not"""
+    M = 1 << 30
+    refused = lambda name, good, **change: _call(name, good, **change) == -1 and b'apart' in lib.load().neurst_last_error()
+    packed = dict(APPEND, k=M + 128, v=M + 192, q=M, q_out=M, k_pages=2 * M, v_pages=3 * M, ldk=128, ldv=128, ldq=128, ldqo=128)      # q | k | v, bf16
+    for change in (dict(k=M), dict(v=M), dict(q_heads=2, q=M + 128, q_out=M + 128), dict(q_heads=2, q=M + 192, q_out=M + 192), dict(k=M + 112),
+                   dict(q=4 * M, q_out=4 * M + 16), dict(q=4 * M, q_out=4 * M + 256 * 3 + 112), dict(q_out=M + 128), dict(q_out=M + 256),
+                   dict(v_pages=2 * M), dict(v_pages=2 * M + 6 * 2 * 16 * 16 * 2 - 16), dict(k_pages=M + 256), dict(v_pages=M + 128), dict(k_pages=M - 16),
+                   dict(q=5 * M, q_out=3 * M), dict(q=2 * M, q_out=2 * M), dict(ldk=136, k=M + 512)):
+        assert refused('neurst_paged_append', packed, **change), change
+    attend = dict(ATTEND, q=M, o=2 * M, k_pages=3 * M, v_pages=4 * M, workspace=5 * M)
+    for change in (dict(o=M), dict(o=M + 128 * 3), dict(o=M + 64, ldq=128, ldo=128), dict(o=3 * M), dict(o=4 * M + 128), dict(workspace=M), dict(workspace=2 * M),
+                   dict(workspace=3 * M + 16), dict(workspace=4 * M), dict(o=5 * M)):
+        assert refused('neurst_paged_attention', attend, **change), change
+    for change in (dict(y=P + 2), dict(y=P + 3 * 64), dict(y=P + 32, ldx=40, ldy=40), dict(y=P + 64, ldx=40, ldy=48)):
+        assert refused('neurst_rotary', ROTARY, **change), change
+
+
 SAMPLE = dict(logits=P, u=P, ids=P, logp=P, t=None, k=None, p=None, m=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, rows=2, V=10, ld=10,
               dtype=0, stream=None)
 
