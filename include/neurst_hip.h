@@ -458,7 +458,9 @@ int neurst_paged_attention(const void* q, const void* k_pages, const void* v_pag
  * (temperature not above 0) or the nearest allowed value.
  * neurst_sample_step draws and keeps a decoding step's books the way neurst_greedy_step does: tokens [rows] = preds[r, step] =
  *   the draw (eos for a finished row or one with nothing to draw), finished |= token == eos, len_decoded += 1 - finished,
- *   n_unfinished += !finished, scores += logp while unfinished. */
+ *   n_unfinished += !finished, scores += logp while unfinished.
+ * neurst_sample_step_checked does the same and ors 4 into *status (may be NULL) when an unfinished row has nothing to draw: it ends
+ *   there with the score it had, which says nothing of it. */
 int neurst_sample(const void* logits, const float* u, int32_t* ids, float* logp, const float* temperature_rows,
                   const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, float temperature, int top_k,
                   float top_p, float min_p, int64_t rows, int64_t V, int64_t ld, int dtype, void* stream);
@@ -467,6 +469,11 @@ int neurst_sample_step(const void* logits, const float* u, int32_t* tokens, int3
                        const int32_t* top_k_rows, const float* top_p_rows, const float* min_p_rows, float temperature,
                        int top_k, float top_p, float min_p, int64_t rows, int64_t V, int64_t ld, int64_t step,
                        int64_t max_steps, int eos, int dtype, void* stream);
+int neurst_sample_step_checked(const void* logits, const float* u, int32_t* tokens, int32_t* preds, int32_t* finished,
+                               int32_t* len_decoded, int32_t* n_unfinished, float* scores, int32_t* status,
+                               const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows,
+                               const float* min_p_rows, float temperature, int top_k, float top_p, float min_p, int64_t rows,
+                               int64_t V, int64_t ld, int64_t step, int64_t max_steps, int eos, int dtype, void* stream);
 
 /* Input pipeline, host side (pure host code, callable without a GPU).  Replaces what the reference
  * gets from TensorFlow's tf.TFRecordReader / tf.parse_single_example / tf.python_io.TFRecordWriter

@@ -33,7 +33,7 @@ struct SampleArgs {
   int32_t* ids;
   float* logp;
   // bookkeeping of a decoding step (all null for a plain draw)
-  int32_t *preds, *finished, *len_decoded, *n_unfinished;
+  int32_t *preds, *finished, *len_decoded, *n_unfinished, *status;
   float* scores;
   int64_t ld, step, max_steps;
   int V, top_k, eos;
@@ -42,6 +42,7 @@ struct SampleArgs {
 
 typedef unsigned long long u64;
 constexpr int SAMPLE_BINS = 1024;
+constexpr int SAMPLE_NOTHING = 4;                    // status: beside the paged cache's 1 and 2
 constexpr double SAMPLE_ONE = 17592186044416.0;      // 2^44
 constexpr float SAMPLE_SPAN = 32.f;                   // e^-32 < 2^-45: rounds to 0
 
@@ -623,6 +624,7 @@ template <typename T, int NT, bool CACHED> __global__ void __launch_bounds__(NT)
         atomicAdd(a.n_unfinished, 1);      // a count: whole numbers, any order
       }
       if (!was && id >= 0) a.scores[row] += logp;
+      if (!was && id < 0 && a.status) atomicOr(a.status, SAMPLE_NOTHING);
       a.ids[row] = tok;
     }
   }
@@ -681,17 +683,26 @@ extern "C" int neurst_sample(const void* logits, const float* u, int32_t* ids, f
   return sample_call(a, rows, V, dtype, stream, "sample");
 }
 
-extern "C" int neurst_sample_step(const void* logits, const float* u, int32_t* tokens, int32_t* preds, int32_t* finished, int32_t* len_decoded,
-                                  int32_t* n_unfinished, float* scores, const float* temperature_rows, const int32_t* top_k_rows,
-                                  const float* top_p_rows, const float* min_p_rows, float temperature, int top_k, float top_p, float min_p,
-                                  int64_t rows, int64_t V, int64_t ld, int64_t step, int64_t max_steps, int eos, int dtype, void* stream) {
+extern "C" int neurst_sample_step_checked(const void* logits, const float* u, int32_t* tokens, int32_t* preds, int32_t* finished,
+                                          int32_t* len_decoded, int32_t* n_unfinished, float* scores, int32_t* status,
+                                          const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows,
+                                          const float* min_p_rows, float temperature, int top_k, float top_p, float min_p, int64_t rows, int64_t V,
+                                          int64_t ld, int64_t step, int64_t max_steps, int eos, int dtype, void* stream) {
   NEURST_CHECK_ARG(tokens && preds && finished && len_decoded && n_unfinished && scores, "sample_step: null pointer");
   NEURST_CHECK_ARG(step >= 0 && step < max_steps, "sample_step: step out of range");
   SampleArgs a = {};
   a.logits = logits; a.u = u; a.ids = tokens; a.preds = preds; a.finished = finished; a.len_decoded = len_decoded;
-  a.n_unfinished = n_unfinished; a.scores = scores;
+  a.n_unfinished = n_unfinished; a.scores = scores; a.status = status;
   a.temperature_rows = temperature_rows; a.top_k_rows = top_k_rows; a.top_p_rows = top_p_rows; a.min_p_rows = min_p_rows;
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.ld = ld;
   a.step = step; a.max_steps = max_steps; a.eos = eos;
   return sample_call(a, rows, V, dtype, stream, "sample_step");
+}
+
+extern "C" int neurst_sample_step(const void* logits, const float* u, int32_t* tokens, int32_t* preds, int32_t* finished, int32_t* len_decoded,
+                                  int32_t* n_unfinished, float* scores, const float* temperature_rows, const int32_t* top_k_rows,
+                                  const float* top_p_rows, const float* min_p_rows, float temperature, int top_k, float top_p, float min_p,
+                                  int64_t rows, int64_t V, int64_t ld, int64_t step, int64_t max_steps, int eos, int dtype, void* stream) {
+  return neurst_sample_step_checked(logits, u, tokens, preds, finished, len_decoded, n_unfinished, scores, nullptr, temperature_rows, top_k_rows,
+                                    top_p_rows, min_p_rows, temperature, top_k, top_p, min_p, rows, V, ld, step, max_steps, eos, dtype, stream);
 }

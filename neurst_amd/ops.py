@@ -825,11 +825,13 @@ def paged_attention_workspace_bytes(tokens, batch, wide, page_size, q_heads, kv_
 
 
 def paged_check(status):
-    """Raises if a kernel found a bad page or length since `status` (int32 [1]) was last zero.  Reads it back: waits."""
+    """Raises if a kernel found a bad page or length, or a decoding step a row with nothing to draw, since `status` (int32 [1])
+    was last zero.  Reads it back: waits."""
     bits = int(status.cpu()[0])
     if bits:
-        raise _lib.NeurstLibError('paged cache: ' + ' and '.join(
-            t for b, t in ((1, 'a page id outside the pool'), (2, 'lengths that do not fit')) if bits & b))
+        raise _lib.NeurstLibError('paged decoding: ' + ' and '.join(
+            t for b, t in ((1, 'a page id outside the pool'), (2, 'lengths that do not fit'),
+                           (4, 'a row of logits with nothing to draw (NaN or -inf throughout)')) if bits & b))
 
 
 # ---- sampling ------------------------------------------------------------------------------------------------------------
@@ -873,8 +875,10 @@ def sample(logits2d, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return ids, logp
 
 
-def sample_step(logits2d, u, tokens, preds, finished, len_decoded, n_unfinished, scores, step, eos, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """The draw of `sample` and the books of a decoding step (neurst_sample_step), as greedy_step keeps them."""
+def sample_step(logits2d, u, tokens, preds, finished, len_decoded, n_unfinished, scores, step, eos, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                status=None):
+    """The draw of `sample` and the books of a decoding step (neurst_sample_step_checked), as greedy_step keeps them.  status: int32
+    [1] for `paged_check`, which then tells of unfinished rows with nothing to draw."""
     dt = dt_of(logits2d)
     R, V, ld, par = _sample_args(logits2d, u, (temperature, top_k, top_p, min_p))
     for t in (tokens, finished, len_decoded):
@@ -886,8 +890,10 @@ def sample_step(logits2d, u, tokens, preds, finished, len_decoded, n_unfinished,
         raise ValueError('sample_step: scores must be fp32 [rows]')
     if n_unfinished.dtype != torch.int32 or n_unfinished.numel() != 1:
         raise ValueError('sample_step: n_unfinished must be one int32')
-    if not _here(logits2d, tokens, preds, finished, len_decoded, n_unfinished, scores):
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError('sample_step: status must be one int32')
+    if not _here(logits2d, tokens, preds, finished, len_decoded, n_unfinished, scores, status):
         raise ValueError('sample_step: every tensor must be on the current GPU')
     if R:
-        _chk(_C.neurst_sample_step(logits2d.data_ptr(), u.data_ptr(), tokens.data_ptr(), preds.data_ptr(), finished.data_ptr(), len_decoded.data_ptr(),
-                                   n_unfinished.data_ptr(), scores.data_ptr(), *par, R, V, ld, step, preds.shape[1], int(eos), dt, _s()), 'sample_step')
+        _chk(_C.neurst_sample_step_checked(logits2d.data_ptr(), u.data_ptr(), tokens.data_ptr(), preds.data_ptr(), finished.data_ptr(), len_decoded.data_ptr(),
+                                           n_unfinished.data_ptr(), scores.data_ptr(), _p(status), *par, R, V, ld, step, preds.shape[1], int(eos), dt, _s()), 'sample_step')

@@ -158,7 +158,7 @@ class Transformer_Decoder(Decoder):
         condition is read every 8 steps as in the greedy loop.
         Returns ([preds [B, num, steps], scores [B, num], lengths [B, num]] with the best score first, best preds [B, steps] int32
         zeroed past their length, their lengths [B]).  preds hold what follows the prefix, scores its log-probability among
-        the words kept at each step."""
+        the words kept at each step.  Raises if a step finds nothing to draw (logits that are NaN or -inf throughout)."""
         g = G.current()
         assert g.tape is None
         s = self.args.sample or {}
@@ -201,7 +201,8 @@ class Transformer_Decoder(Decoder):
         step = 0
         while step < max_steps:
             logits = run.step(cur, step)
-            ops.sample_step(logits, us[step], tokens, preds, finished, len_decoded, unfinished_hist[step:step + 1], scores, step, int(self.end_token), **rule)
+            ops.sample_step(logits, us[step], tokens, preds, finished, len_decoded, unfinished_hist[step:step + 1], scores, step, int(self.end_token),
+                            status=run.status, **rule)
             cur = tokens
             step += 1
             if step % CHECK_EVERY == 0 or step == max_steps:

@@ -746,6 +746,33 @@ def test_sample_step_keeps_the_books():
     np.testing.assert_allclose(scores.cpu().numpy(), ps, rtol=0, atol=steps * 2.0 ** -22 * 8)
 
 
+def test_sample_step_tells_of_rows_with_nothing_to_draw():
+    """an unfinished row of NaN and -inf raises the status, a finished one does not; the books are the same without it"""
+    R, V, eos = 6, 70, 3
+    x = normal(gen(97), R, V)
+    u = torch.full((R,), 0.5, device=DEV)
+
+    def step(x, done, status):
+        preds, left = torch.zeros(R, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+        tokens, ln = (torch.zeros(R, dtype=torch.int32, device=DEV) for _ in range(2))
+        fin, scores = i32([int(r in done) for r in range(R)]), torch.zeros(R, device=DEV)
+        ops.sample_step(x, u, tokens, preds, fin, ln, left, scores, 0, eos, status=status)
+        return tokens, preds, fin, ln, left, scores
+    for value in (float('nan'), -float('inf')):
+        bad = x.clone()
+        bad[4] = value
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        for logits, done, bits in ((x, (), 0), (x, (1,), 0), (bad, (4,), 0), (bad, (), 4)):
+            status.zero_()
+            got = step(logits, done, status)
+            assert int(status) == bits, (value, done)
+            assert all(torch.equal(a, b) for a, b in zip(got, step(logits, done, None)))
+        with pytest.raises(lib.NeurstLibError, match='nothing to draw'):
+            ops.paged_check(status)
+    with pytest.raises(ValueError, match='status'):
+        step(x, (), torch.zeros(2, dtype=torch.int32, device=DEV))
+
+
 # ---- a run of them together --------------------------------------------------------------------------------------------------------
 def decode_run(g, dtype, steps=5, graph=False):
     """a forced prefix for three sequences, then single tokens: rotary -> append -> attention -> logits -> draw, against the

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import __graft_entry__ as ge
-from neurst_amd import ops
+from neurst_amd import lib, ops
 from neurst_amd.synthetic import make_batch
 
 pytestmark = pytest.mark.gpu
@@ -97,6 +97,18 @@ def test_draws_repeat_with_their_seed_and_differ_without():
     m.infer(*feats)
     assert not np.array_equal(one[1][0], m.last['samples'][0])
     assert (one[1][0] >= 0).all() and (one[1][0] < 11).all()
+
+
+def test_logits_that_are_nan_are_not_a_translation():
+    """a hypothesis that breaks off keeps the score it had, the best there is: the call raises instead of returning it"""
+    args, m, feats = make_model(4, decode='sample', sample=dict(num=2, seed=3))
+    m.infer(*feats)
+    P = m.store.export()
+    fc = [k for k in P if k.endswith('decoder_fc/kernel')][0]
+    P[fc][:] = np.nan
+    m.store.load_params(P)
+    with pytest.raises(lib.NeurstLibError, match='nothing to draw'):
+        m.infer(*feats)
 
 
 def test_refusals():

@@ -121,6 +121,15 @@ def test_sample_step_refuses():
         assert _call('neurst_sample_step', good, **change) == -1, change
 
 
+def test_sample_step_checked_refuses():
+    good = dict(logits=P, u=P, tokens=P, preds=P, finished=P, len_decoded=P, n_unfinished=P, scores=P, status=P, t=None, k=None, p=None, m=None,
+                temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, rows=2, V=10, ld=10, step=0, max_steps=4, eos=3, dtype=0, stream=None)
+    for change in [{k: None} for k in ('logits', 'tokens', 'preds', 'finished', 'len_decoded', 'n_unfinished', 'scores', 'u')] + [
+            dict(step=4), dict(step=-1), dict(top_p=2.0), dict(ld=9), dict(dtype=2)]:
+        assert _call('neurst_sample_step_checked', good, **change) == -1, change
+    assert _call('neurst_sample_step_checked', good, rows=0) == 0
+
+
 def test_calls_without_rows_do_nothing():
     assert _call('neurst_rotary', ROTARY, rows=0) == 0
     assert _call('neurst_paged_append', APPEND, tokens=0) == 0
