@@ -23,8 +23,8 @@ def demangle(n):
 
 def scan(path):
     with tempfile.NamedTemporaryFile(suffix='.s') as tmp:
-        subprocess.run(['hipcc', '-O3', '--offload-arch=gfx950', '-std=c++17', '-Wno-unused-value', '-S', '--cuda-device-only', path, '-o', tmp.name],
-                       check=True, stderr=subprocess.DEVNULL, cwd=SRC)
+        compiler = subprocess.run(['make', '-s', 'flags'], check=True, capture_output=True, text=True, cwd=SRC).stdout.split()      # as it is shipped
+        subprocess.run(compiler + ['-S', '--cuda-device-only', path, '-o', tmp.name], check=True, stderr=subprocess.DEVNULL, cwd=SRC)
         text = open(tmp.name).read()
     out = []
     for f in re.split(r'\n(?=_Z\w+:\s)', text):
