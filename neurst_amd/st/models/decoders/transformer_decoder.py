@@ -22,6 +22,7 @@ class Transformer_Decoder(Decoder):
         self.residual_dropout_rate = d.residual_dropout_rate if is_train else 0.0
         self.num_heads = d.num_heads
         self.size_embedding = d.size_embedding
+        self.draws = None
 
     def rotary(self, device):
         return Rotary.of(self.args.model.decoder.rotary, self.num_cell_units // self.num_heads, device)
@@ -151,8 +152,8 @@ class Transformer_Decoder(Decoder):
 
     def sample_decode(self, encoded, len_encoded, prefix=None, len_prefix=None):
         """Draws `sample.num` translations per utterance: rows are (utterance b, sample j) = b * num + j.  The YAML mapping
-        `sample`: num (1), temperature (1.0; 0: the arg-max), top_k (0: all), top_p (1.0), min_p (0.0), seed (the model's),
-        page_size (16).  prefix int [B, Lp] and len_prefix int [B] (numpy or torch): tokens every translation of an utterance
+        `sample`: num (1), temperature (1.0; 0: the arg-max), top_k (0: all), top_p (1.0), min_p (0.0), seed (every call draws
+        anew from it; without it the draws go on from call to call, the first from the model's seed), page_size (16).  prefix int [B, Lp] and len_prefix int [B] (numpy or torch): tokens every translation of an utterance
         begins with; they enter the cache as one chunk, behind <sos>.  The steps run over a paged cache (each row its own
         pages for its tokens, the utterance's pages with the encoder-side keys and values shared by its samples); the stop
         condition is read every 8 steps as in the greedy loop.
@@ -191,8 +192,7 @@ class Transformer_Decoder(Decoder):
         first = [np.concatenate([[self.start_token], prefix[b, :lp[b]] if lp[b] else []]).astype(np.int32) for b in range(B) for _ in range(num)]
         lens = np.repeat(lp, num) + 1                                      # tokens of the first chunk
         run = _PagedDecoderStep(self, encoded, len_encoded, num, lens, max_steps, page)
-        gen = torch.Generator(device=dev).manual_seed(int(get('seed', self.args.seed or 0)))
-        us = torch.rand((max_steps, R), generator=gen, device=dev)
+        us = torch.rand((max_steps, R), generator=self._draws(get('seed', None), dev), device=dev)
         zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)
         preds, tokens, finished, unfinished_hist = zeros(R, max_steps), zeros(R), zeros(R), zeros(max_steps)
         len_decoded, scores = torch.ones(R, dtype=torch.int32, device=dev), torch.zeros(R, dtype=torch.float32, device=dev)
@@ -219,6 +219,14 @@ class Transformer_Decoder(Decoder):
         pick = lambda x: np.take_along_axis(x, order.reshape(order.shape + (1,) * (x.ndim - 2)), 1)
         out, sc, ld = pick(out), pick(sc), pick(ld)
         return [out, sc, ld], out[:, 0, :], ld[:, 0]
+
+    def _draws(self, seed, dev):
+        """a generator that begins anew from a given seed, or the decoder's own, which goes on from call to call"""
+        if seed is not None:
+            return torch.Generator(device=dev).manual_seed(int(seed))
+        if self.draws is None or self.draws.device != dev:
+            self.draws = torch.Generator(device=dev).manual_seed(int(self.args.seed or 0))
+        return self.draws
 
     @staticmethod
     def _beam_result(preds, scores, len_decoded, finished, step, B, K):

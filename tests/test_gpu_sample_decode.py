@@ -99,6 +99,24 @@ def test_draws_repeat_with_their_seed_and_differ_without():
     assert (one[1][0] >= 0).all() and (one[1][0] < 11).all()
 
 
+def test_calls_without_a_seed_draw_numbers_of_their_own():
+    """two batches of a test set are not drawn with the same numbers; a new model repeats the run"""
+    runs = []
+    for _ in range(2):
+        args, m, feats = make_model(8, decode='sample', sample=dict(num=3, temperature=1.5))
+        runs.append([])
+        for _ in range(2):
+            m.infer(*feats)
+            runs[-1].append(m.last['samples'])
+    assert all(np.array_equal(x, y) for a, b in zip(*runs) for x, y in zip(a, b))
+    assert not np.array_equal(runs[0][0][1], runs[0][1][1])
+    args.sample = dict(args.sample, seed=5)
+    m.infer(*feats)
+    seeded = m.last['samples']
+    m.infer(*feats)
+    assert all(np.array_equal(x, y) for x, y in zip(seeded, m.last['samples']))
+
+
 def test_logits_that_are_nan_are_not_a_translation():
     """a hypothesis that breaks off keeps the score it had, the best there is: the call raises instead of returning it"""
     args, m, feats = make_model(4, decode='sample', sample=dict(num=2, seed=3))
