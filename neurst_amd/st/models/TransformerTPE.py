@@ -517,7 +517,7 @@ class TransformerTPE(Seq2SeqModel):
         a = self.args
         if a.decode not in (None, 'search', 'sample'):
             raise ValueError("decode must be 'search' (greedy, or beam with beam_size > 1) or 'sample'")
-        if prefix is not None and a.decode != 'sample':
+        if (prefix is not None or len_prefix is not None) and a.decode != 'sample':
             raise NotImplementedError("a forced prefix needs decode: sample (with sample.temperature 0 it is the greedy search)")
         if a.dirs and a.dirs.lm_checkpoint:
             raise NotImplementedError('LM rerank (dirs.lm_checkpoint) is outside the hot path')

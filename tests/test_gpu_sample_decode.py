@@ -129,6 +129,12 @@ def test_logits_that_are_nan_are_not_a_translation():
         m.infer(*feats)
 
 
+def test_lengths_of_a_prefix_need_sampled_decoding():
+    args, m, feats = make_model(9)
+    with pytest.raises(NotImplementedError, match='prefix'):
+        m.infer(*feats, len_prefix=np.array([0, 0, 0]))
+
+
 def test_refusals():
     args, m, feats = make_model(9, decode='sample', sample=dict(nmu=3))
     with pytest.raises(ValueError, match='unknown keys'):
