@@ -39,7 +39,7 @@ __device__ __forceinline__ void paged_look_over(const PagedIndex& x, int32_t* st
 #define PAGED_CHECK_INDEX(name)                                                                                            \
   NEURST_CHECK_ARG(page_table && cu_new && ctx_len, name ": null index pointer");                                           \
   NEURST_CHECK_ARG(tokens >= 0 && tokens <= INT32_MAX && batch >= 0 && batch <= (1 << 20), name ": bad token or sequence count"); \
-  NEURST_CHECK_ARG(n_pages > 0 && n_pages <= INT32_MAX && wide > 0 && (ld_table >= wide || ld_table == 0), name ": bad page counts");          \
+  NEURST_CHECK_ARG(n_pages > 0 && n_pages <= INT32_MAX && wide > 0 && wide <= INT32_MAX && (ld_table >= wide || ld_table == 0), name ": bad page counts");          \
   NEURST_CHECK_ARG(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,                              \
                    name ": page_size must be a power of two in 16..4096");                                                  \
   NEURST_CHECK_ARG(wide * page_size <= INT32_MAX - 4096, name ": a sequence is limited to 2^31 - 4097 positions");          \

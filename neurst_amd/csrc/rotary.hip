@@ -78,7 +78,9 @@ extern "C" int neurst_rotary(const void* x, void* y, const double* freq, const i
   NEURST_CHECK_ARG(layout == ROT_HALF || layout == ROT_INTERLEAVED, "rotary: layout must be 0 (half) or 1 (interleaved)");
   NEURST_CHECK_ARG(x != y || ldx == ldy, "rotary: in place needs equal row strides");
   NEURST_CHECK_ARG(period >= 0 && period <= INT32_MAX, "rotary: bad period");
-  NEURST_CHECK_ARG(positions || (pos0 >= INT32_MIN && pos0 + (period ? period : rows) <= INT32_MAX), "rotary: positions must fit 32 bits");
+  NEURST_CHECK_ARG(heads * dh <= INT32_MAX, "rotary: rows are limited to 2^31 - 1 columns");
+  NEURST_CHECK_ARG(positions || (pos0 >= INT32_MIN && pos0 <= INT32_MAX && pos0 <= INT32_MAX - (period ? period : rows)),
+                   "rotary: positions must fit 32 bits");
   const int64_t es = (int64_t)dtype_size(dtype);
   if (layout == ROT_INTERLEAVED)
     NEURST_CHECK_ARG((((uintptr_t)x | (uintptr_t)y | (uintptr_t)(ldx * es) | (uintptr_t)(ldy * es) | (uintptr_t)(dh * es)) % (2 * es)) == 0,

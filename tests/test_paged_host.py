@@ -121,6 +121,16 @@ def test_sample_step_refuses():
         assert _call('neurst_sample_step', good, **change) == -1, change
 
 
+def test_sizes_that_pass_64_bits_are_refused():
+    """sums and products of the checks themselves"""
+    for change in (dict(positions=None, pos0=2 ** 63 - 1), dict(positions=None, pos0=2 ** 63 - 1, period=7), dict(positions=None, rows=2 ** 62, pos0=-2 ** 31),
+                   dict(heads=65536, dh=65536, pairs=1, ldx=2 ** 32, ldy=2 ** 32)):
+        assert _call('neurst_rotary', ROTARY, **change) == -1, change
+    for name, good in (('neurst_paged_append', APPEND), ('neurst_paged_attention', dict(ATTEND, workspace=None))):
+        assert _call(name, good, wide=2 ** 60, ld_table=2 ** 60) == -1
+        assert b'bad page counts' in lib.load().neurst_last_error()
+
+
 def test_sample_step_checked_refuses():
     good = dict(logits=P, u=P, tokens=P, preds=P, finished=P, len_decoded=P, n_unfinished=P, scores=P, status=P, t=None, k=None, p=None, m=None,
                 temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, rows=2, V=10, ld=10, step=0, max_steps=4, eos=3, dtype=0, stream=None)
