@@ -912,7 +912,7 @@ extern "C" int neurst_paged_attention(const void* q, const void* k_pages, const 
   NEURST_CHECK_ARG((tokens * (q_heads / kv_heads) / 16 + batch) * kv_heads <= INT32_MAX && tokens * (q_heads / kv_heads) <= INT32_MAX,
                    "paged_attention: too many rows");
   NEURST_CHECK_ARG(ldq >= q_heads * dh && ldo >= q_heads * dh, "paged_attention: a row stride is smaller than its heads");
-  NEURST_CHECK_ARG(scale == scale && scale <= 3.4e38f && scale >= -3.4e38f, "paged_attention: scale must be finite");
+  NEURST_CHECK_ARG(fabsf(scale) <= 2.3e38f, "paged_attention: scale must be finite, and so must scale * log2(e)");
   const int64_t es = (int64_t)dtype_size(dtype);
   const uintptr_t align = (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o | (uintptr_t)(ldq * es) | (uintptr_t)(ldo * es);
   NEURST_CHECK_ARG(align % 16 == 0, "paged_attention: pointers and row strides must be 16-byte aligned");

@@ -786,7 +786,7 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_new, ctx_len, scale=None
     if q.dim() != 3 or q.shape[2] != dh or q.dtype != k_pages.dtype:
         raise ValueError('paged_attention: q must be [tokens, q_heads, dh] of the type of the pages')
     tokens, qh = q.shape[0], q.shape[1]
-    if qh == 0 or qh % kvh:
+    if qh == 0 or kvh == 0 or qh % kvh:
         raise ValueError('paged_attention: q heads must be a multiple of the key / value heads')
     ldq = _row_stride(q, qh, dh)
     if ldq < 0:

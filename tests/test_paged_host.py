@@ -131,6 +131,15 @@ def test_sizes_that_pass_64_bits_are_refused():
         assert b'bad page counts' in lib.load().neurst_last_error()
 
 
+def test_scales_and_head_counts_at_their_limits_are_refused():
+    for scale in (3.3e38, -3.3e38, 2.4e38, NAN, -INF):      # times log2(e) beyond fp32
+        assert _call('neurst_paged_attention', ATTEND, scale=scale) == -1
+        assert b'scale' in lib.load().neurst_last_error()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    with pytest.raises(ValueError, match='heads'):
+        ops.paged_attention(torch.zeros(3, 2, 8), torch.zeros(4, 0, 16, 8), torch.zeros(4, 0, 8, 16), torch.zeros(2, 1, dtype=torch.int32), i32(0, 1, 3), i32(1, 2))
+
+
 def test_sample_step_checked_refuses():
     good = dict(logits=P, u=P, tokens=P, preds=P, finished=P, len_decoded=P, n_unfinished=P, scores=P, status=P, t=None, k=None, p=None, m=None,
                 temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, rows=2, V=10, ld=10, step=0, max_steps=4, eos=3, dtype=0, stream=None)
