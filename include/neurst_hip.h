@@ -409,7 +409,8 @@ int neurst_gather_rows(const void* src, void* dst, const int32_t* idx, int64_t r
  * over it, drawing the next token. ----
  *
  * Rotary positions: y = x with the first 2 * pairs columns of each head turned by the row's position.  Pair i at position p:
- *   u' = mscale (u cos a - v sin a), v' = mscale (v cos a + u sin a), a = p * freq[i] (fp64 inside: exact to 2^-33 turns),
+ *   u' = mscale (u cos a - v sin a), v' = mscale (v cos a + u sin a), a = p * freq[i] (good to
+ *   |a| 2^-54 + 2^-26 turns),
  * the pair being columns (i, pairs + i) (layout 0, "half") or (2 i, 2 i + 1) (layout 1, "interleaved"); further columns
  * pass through.  x, y: rows of `heads` heads of dh columns at row strides ldx / ldy (elements); y may be x.  positions
  * int32 [rows], or NULL: row r stands at pos0 + (period ? r % period : r).  inverse != 0 turns back: the gradient. */
@@ -424,9 +425,13 @@ int neurst_rotary(const void* x, void* y, const double* freq, const int32_t* pos
  * sequence b owns rows cu_new[b] .. cu_new[b + 1] - 1 (none is fine); ctx_len int32 [batch] = tokens in its cache WITH them, so
  * its row j stands at position ctx_len[b] - n_b + j.  Rows of no sequence are left as they are.
  *
- * These arrays live on the device.  A kernel that finds lengths that do not fit (rows out of range, ctx_len beyond the
- * table, or below n_b unless attention is not causal) or a page id outside the pool leaves that sequence or those keys out, and ors 2 or 1 into *status (may
- * be NULL); it reads and writes nothing out of range.
+ * These arrays live on the device.  What does not fit is left out, told by a bit ored into *status (may be NULL), and nothing is
+ * read or written out of range:
+ *   2: rows out of range or cu_new falling - the sequence's rows stay as they are, and where cu_new falls other sequences may
+ *      lose rows too; ctx_len beyond the table, or below n_b unless attention is not causal - nothing is appended, attention
+ *      gives zeros;
+ *   1: a page id outside the pool - its keys are neither written nor seen.
+ * What a call writes (pages, q_out, o, workspace) must be apart from all it reads, but for q_out = q.
  *
  * neurst_paged_append writes the new keys k (rotated by position when freq is not NULL: pairs, layout, mscale as above) and
  *   values v into their pages and, when q is not NULL, the rotated queries to q_out (may be q).

@@ -7,8 +7,8 @@
 // 16-byte load from the page, with no trip through shared memory.  The price is paid here, once per token: a chunk is
 // transposed in registers eight slots at a time, a single token scatters dh elements of 2 bytes.
 //
-// Bound by memory (chunks: 37 sequences of up to 700 tokens, 8 heads of 64 columns, bf16, 30 us = 3.5 TB/s - the transposition
-// reads and writes 128-byte pieces) or by the launch (64 single tokens of 96 columns: 5.0 us).  A tile is 64 positions aligned in the cache; its items - 16
+// Bound by memory (chunks: 37 sequences of up to 700 tokens, 8 heads of 64 columns, bf16, 30 to 33 us = 3.2 to 3.5 TB/s at pages of
+// 32 slots and more, 36 at 16; fp32 47 us = 4.5 TB/s at any) or by the launch (64 single tokens of 96 columns: 5.0 us).  A tile is 64 positions aligned in the cache; its items - 16
 // bytes of a query or key row with its partner of the pair, eight slots x eight columns of values - are dealt to
 // gridDim.y workgroups.  Lanes of a value item run over the slot groups first, then over the columns: a wave reads whole
 // 128-byte row pieces and writes whole 128-byte column pieces.

@@ -12,16 +12,17 @@
 // instruction such that a lane's results are eight CONSECUTIVE keys of one query: after exp2 and the rounding to bf16 they
 // are, in place, the operand of O^T = V^T P^T, whose other operand is one 16-byte load from the transposed value pages.  No
 // shared memory and no barrier until the waves join their partial results.  Bound by the cache's bytes: 32 sequences of up to
-// 32000 keys, 32 heads on 8 of 128 columns, bf16, 396 us = 5.2 TB/s (a large copy here: 4.8).  Short ones by the chain lengths -
-// page - keys - exponentials - values - join: 8 sequences of up to 500 keys, 8 heads of 64 columns, 7.0 us; 13 chunks of up to
-// 75 tokens over 611 keys in fp32 23 us.
+// 32000 keys, 32 heads on 8 of 128 columns, bf16, 396 to 411 us = 5.0 to 5.2 TB/s (a large copy here: 4.8).  Short ones by the chain lengths -
+// page - keys - exponentials - values - join: 8 sequences of up to 500 keys, 8 heads of 64 columns, 6.9 us; 13 chunks of up to
+// 75 tokens over 611 keys in fp32 24 us.
 //
 // paged_attn_tiles: many rows, bf16.  A wave owns 32 rows, a workgroup NW of them; tiles of 64 keys go from the pages to shared
 // memory by direct loads, one tile ahead of the one in use, and all waves read them from there.  The same transposed
 // products with the 32 x 32 x 16 instruction; the key that sits in row r of a 32-key block is chosen again so that a lane's
 // results are runs of eight consecutive keys.  The first product of a tile runs beside the exponentials of the tile before,
 // the second beside the next maximum.  Bound by what a CU's matrix, vector and shared-memory pipes do not overlap: three
-// sequences of up to 4096 rows over 9000 keys, 16 heads on 4 of 128 columns, 508 us = 834 TFLOP/s (a large product: 1673).
+// sequences of up to 4096 rows over 9000 keys, 16 heads on 4 of 128 columns, 500 to 526 us = 806 to 848 TFLOP/s (a large
+// product: 1673); the first twenty calls after a pause take 550 to 610 us, until the card's clocks have settled.
 // With any one of them left out it would still take four fifths: without the loads 78 %, without reading shared memory 83 %,
 // without the exponentials 87 %.
 #include "paged.h"
@@ -520,7 +521,8 @@ __global__ void __launch_bounds__(TILE_WAVES * 64, DH <= 128 ? 2 : 1) paged_attn
   };
 
   // Software pipeline, a tile t at a time: the first product of tile t + 1 runs while the vector unit makes the weights of
-  // tile t, the second product of t while it finds the maximum of t + 1.  Keys are loaded two tiles ahead, values one.
+  // tile t, the second product of t while it finds the maximum of t + 1.  The keys of t + 2 and the values of t + 1 are loaded on the
+  // way: both are used in the next turn, which begins with waiting for them.
   const int t1w = (w_end + KT - 1) / KT < t1 ? (w_end + KT - 1) / KT : t1;      // the wave's own end
   int id0 = pages_of(t0), id1 = pages_of(t0 + 1), id2 = pages_of(t0 + 2);
   f32x16 s[2];

@@ -22,7 +22,8 @@
 // One workgroup a row; a row of up to 132 KB is read once, into shared memory, and every later pass runs on that.  Bound by
 // the chain of passes and barriers: one row of 10000 words with top_p takes 13 us (its arg-max alone 4.0), 256 rows of 32003
 // words with every filter, a CU each, 22 us = 1.5 TB/s (the arg-max 9.4 = 3.5 TB/s); without top_k by the fp64 exponentials,
-// some 26 instructions a word: 256 rows of 32003 with top_p alone 28 us.
+// some 26 instructions a word: 256 rows of 32003 with top_p alone 28 us.  Longer rows are read from memory again by every pass:
+// one row of 128000 words takes 41 us for the arg-max, 71 with every filter, 137 with top_p alone; 256 of them 116, 180, 289.
 #include "common.h"
 
 struct SampleArgs {
